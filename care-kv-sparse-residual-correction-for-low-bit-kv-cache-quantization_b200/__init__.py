@@ -13,6 +13,9 @@ from .quantizer import (QuantConfig, KQuantizer, VQuantizer, quantize, dequantiz
                         pack_int2_2d, unpack_int2_2d, pack_int3_2d, unpack_int3_2d, pack_int4_2d, unpack_int4_2d,
                         pack_codes_2d, unpack_codes_2d, packed_row_bytes, pack_4bit, unpack_4bit,
                         quant_dequant_kivi_k, quant_dequant_kivi_v)
+from .rotary import RotaryEmbedding, apply_rotary, rotary_frequencies
+from .weights import PackedWeight
+from .prefix import SharedPrefix, prefix_attention
 from .engine import DecodeEngine
 from .layer import CAREKVLayer, causal_attention, resolve_prefill_mode
 from .llama_patch import CAREKVLlamaAttention, patch_llama_model, reset_all_caches
@@ -27,6 +30,7 @@ __all__ = [
     "pack_int2_2d", "unpack_int2_2d", "pack_int3_2d", "unpack_int3_2d", "pack_int4_2d", "unpack_int4_2d",
     "pack_codes_2d", "unpack_codes_2d", "packed_row_bytes", "pack_4bit", "unpack_4bit",
     "quant_dequant_kivi_k", "quant_dequant_kivi_v",
+    "RotaryEmbedding", "apply_rotary", "rotary_frequencies", "PackedWeight", "SharedPrefix", "prefix_attention",
     "DecodeEngine", "CAREKVLayer", "causal_attention", "resolve_prefill_mode",
     "CAREKVLlamaAttention", "patch_llama_model", "reset_all_caches", "CAREKVAdapter",
 ]

@@ -72,6 +72,25 @@ class Shard(ctypes.Structure):
     _fields_ = [("kvh_begin", i32), ("kvh_total", i32)]
 
 
+class Rows(ctypes.Structure):
+    _fields_ = [("in_", vp), ("out", vp), ("in_stride", i64 * 3), ("out_stride", i64 * 3), ("heads", i32)]
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = [("q", Rows), ("k", Rows), ("freq", vp), ("positions", vp), ("position_stride", i64 * 2),
+                ("position_bytes", i32), ("batch", i32), ("tokens", i32), ("head_dim", i32), ("rotary_dim", i32),
+                ("interleaved", i32), ("inverse", i32), ("factor", f32), ("dtype", i32)]
+
+
+class W4(ctypes.Structure):
+    _fields_ = [("codes", vp), ("scales", vp), ("n", i32), ("k", i32), ("group_size", i32), ("dtype", i32)]
+
+
+class Prefix(ctypes.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("k_stride", i64 * 2), ("v_stride", i64 * 2), ("num_kv_heads", i32),
+                ("tokens", i32), ("head_dim", i32), ("dtype", i32)]
+
+
 # (name, restype, argtypes) of every exported symbol declared in the header
 SIGNATURES = [
     ("carekv_abi_version", i32, []),
@@ -108,6 +127,14 @@ SIGNATURES = [
     ("carekv_decode_attention_shard", i32, [ctypes.POINTER(Config), ctypes.POINTER(Cache), i32, vp, vp, i32, i32,
                                             i32, i32, ctypes.POINTER(RouteParams), vp, vp, ctypes.c_size_t,
                                             ctypes.POINTER(Shard), vp]),
+    ("carekv_rotary", i32, [ctypes.POINTER(Rotary), vp]),
+    ("carekv_w4_layout", i32, [ctypes.POINTER(W4), ctypes.POINTER(ctypes.c_size_t)]),
+    ("carekv_w4_pack", i32, [ctypes.POINTER(W4), vp, vp, vp]),
+    ("carekv_w4_dequantize", i32, [ctypes.POINTER(W4), vp, vp]),
+    ("carekv_w4_matvec", i32, [ctypes.POINTER(W4), vp, i64, i32, vp, vp]),
+    ("carekv_prefix_workspace_bytes", i32, [ctypes.POINTER(Prefix), i32, i32, ctypes.POINTER(ctypes.c_size_t)]),
+    ("carekv_prefix_attention", i32, [ctypes.POINTER(Prefix), vp, i64, i64, i32, i32, f32, vp, vp, vp, vp, vp, vp,
+                                      ctypes.c_size_t, vp]),
 ]
 NOALLOC_MAX_BYTES = 64 << 20
 

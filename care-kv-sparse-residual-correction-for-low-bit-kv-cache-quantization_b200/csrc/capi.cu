@@ -1,5 +1,6 @@
 // extern "C" entry points of libcarekv_b200.so: argument validation, buffer
 // layout and launch.  See include/carekv_b200.h for the contract of each.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -406,6 +407,92 @@ int carekv_decode_attention_launches(const carekv_config_t* cfg, int32_t seq_cou
   if (!launches || seq_count < 0) return CAREKV_ERR_INVALID_ARG;
   *launches = 2 * decode_attention_chunks(seq_count);
   return CAREKV_OK;
+}
+
+int carekv_rotary(const carekv_rotary_t* a, void* stream) {
+  if (!a || !a->freq || a->batch < 0 || a->tokens < 0 || a->q.heads < 0 || a->k.heads < 0) return CAREKV_ERR_INVALID_ARG;
+  if (a->head_dim < 1 || a->rotary_dim < 2 || a->rotary_dim % 2 || a->rotary_dim > a->head_dim)
+    return CAREKV_ERR_INVALID_ARG;
+  if (a->head_dim > 256) return CAREKV_ERR_UNSUPPORTED;
+  if (a->position_bytes != 4 && a->position_bytes != 8) return CAREKV_ERR_INVALID_ARG;
+  CHECK(validate_dtype(a->dtype));
+  const int64_t tok = static_cast<int64_t>(a->batch) * a->tokens;
+  if (tok > INT32_MAX || tok * (static_cast<int64_t>(a->q.heads) + a->k.heads) > (int64_t{1} << 40))
+    return CAREKV_ERR_UNSUPPORTED;
+  if (tok == 0) return CAREKV_OK;
+  if (!a->positions) return CAREKV_ERR_INVALID_ARG;
+  for (const carekv_rows_t* r : {&a->q, &a->k})
+    if (r->heads > 0 && (!r->in || !r->out || r->in == r->out)) return CAREKV_ERR_INVALID_ARG;
+  return cuda_status(launch_rotary(*a, as_stream(stream)));
+}
+
+static int validate_w4(const carekv_w4_t* w) {
+  if (!w || w->n < 1 || w->k < 1 || w->group_size < 1 || w->k % w->group_size) return CAREKV_ERR_INVALID_ARG;
+  if (w->group_size != 32 && w->group_size != 64 && w->group_size % 128) return CAREKV_ERR_UNSUPPORTED;
+  return validate_dtype(w->dtype);
+}
+static int validate_w4_buffers(const carekv_w4_t* w) {
+  CHECK(validate_w4(w));
+  if (!w->codes || !w->scales) return CAREKV_ERR_INVALID_ARG;
+  const uintptr_t m = reinterpret_cast<uintptr_t>(w->codes) | reinterpret_cast<uintptr_t>(w->scales);
+  return (m & 15) ? CAREKV_ERR_INVALID_ARG : CAREKV_OK;
+}
+
+int carekv_w4_layout(const carekv_w4_t* w, size_t sizes[2]) {
+  CHECK(validate_w4(w));
+  if (!sizes) return CAREKV_ERR_INVALID_ARG;
+  w4_layout(w->n, w->k, w->group_size, w->dtype, sizes);
+  return CAREKV_OK;
+}
+
+int carekv_w4_pack(const carekv_w4_t* w, const void* packed, const void* scale, void* stream) {
+  CHECK(validate_w4_buffers(w));
+  if (!packed || !scale) return CAREKV_ERR_INVALID_ARG;
+  return cuda_status(launch_w4_pack(packed, scale, *w, w->codes, w->scales, as_stream(stream)));
+}
+
+int carekv_w4_dequantize(const carekv_w4_t* w, void* out, void* stream) {
+  CHECK(validate_w4_buffers(w));
+  if (!out) return CAREKV_ERR_INVALID_ARG;
+  return cuda_status(launch_w4_dequant(*w, out, as_stream(stream)));
+}
+
+int carekv_w4_matvec(const carekv_w4_t* w, const void* x, int64_t x_stride, int32_t rows, void* out, void* stream) {
+  CHECK(validate_w4_buffers(w));
+  if (rows < 0) return CAREKV_ERR_INVALID_ARG;
+  if (rows == 0) return CAREKV_OK;
+  if (!x || !out || x_stride < w->k) return CAREKV_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(x) & 15) || (x_stride * act_bytes(w->dtype)) % 16) return CAREKV_ERR_INVALID_ARG;
+  return cuda_status(launch_w4(*w, x, x_stride, rows, out, as_stream(stream)));
+}
+
+static int validate_prefix(const carekv_prefix_t* p, int32_t rows, int32_t heads) {
+  if (!p || p->num_kv_heads < 1 || p->tokens < 0 || p->head_dim < 1 || rows < 0 || heads < 1) return CAREKV_ERR_INVALID_ARG;
+  if (heads % p->num_kv_heads) return CAREKV_ERR_INVALID_ARG;
+  if (p->head_dim > 256 || p->num_kv_heads > 65535 || static_cast<int64_t>(rows) * heads > INT32_MAX)
+    return CAREKV_ERR_UNSUPPORTED;
+  return validate_dtype(p->dtype);
+}
+
+int carekv_prefix_workspace_bytes(const carekv_prefix_t* p, int32_t rows, int32_t heads, size_t* bytes) {
+  CHECK(validate_prefix(p, rows, heads));
+  if (!bytes) return CAREKV_ERR_INVALID_ARG;
+  *bytes = prefix_workspace_bytes(*p, rows, heads);
+  return CAREKV_OK;
+}
+
+int carekv_prefix_attention(const carekv_prefix_t* p, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                            int32_t rows, int32_t heads, float scale, const int32_t* lengths, const void* tail_out,
+                            const float* tail_lse, void* out, float* lse, void* ws, size_t ws_bytes, void* stream) {
+  CHECK(validate_prefix(p, rows, heads));
+  if (rows == 0) return CAREKV_OK;
+  if (!q || !out || (p->tokens > 0 && (!p->k || !p->v))) return CAREKV_ERR_INVALID_ARG;
+  if ((tail_out == nullptr) != (tail_lse == nullptr)) return CAREKV_ERR_INVALID_ARG;
+  const size_t need = prefix_workspace_bytes(*p, rows, heads);
+  if (need > 0 && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15))) return CAREKV_ERR_INVALID_ARG;
+  if (ws_bytes < need) return CAREKV_ERR_WORKSPACE;
+  return cuda_status(launch_prefix(*p, q, q_row_stride, q_head_stride, rows, heads, scale, lengths, tail_out, tail_lse,
+                                   out, lse, ws, as_stream(stream)));
 }
 
 int carekv_check_device_errors(const carekv_cache_t* cache, int32_t* flags_out, void* stream) {

@@ -31,6 +31,16 @@ cudaError_t launch_append(const carekv_config_t& cfg, const carekv_cache_t& cach
                           const float* sketch_proj, int may_fill, int in_H, cudaStream_t st);
 cudaError_t launch_kivi_k(const void* x, void* out, int64_t n, int T, int D, int bits, int dt, cudaStream_t st);
 cudaError_t launch_kivi_v(const void* x, void* out, int64_t rows, int D, int bits, int dt, cudaStream_t st);
+cudaError_t launch_rotary(const carekv_rotary_t& a, cudaStream_t st);
+void w4_layout(int n, int k, int group, int dt, size_t sizes[2]);
+cudaError_t launch_w4_pack(const void* packed, const void* scale, const carekv_w4_t& w, void* codes, void* scales,
+                           cudaStream_t st);
+cudaError_t launch_w4_dequant(const carekv_w4_t& w, void* out, cudaStream_t st);
+cudaError_t launch_w4(const carekv_w4_t& w, const void* x, int64_t ldx, int M, void* out, cudaStream_t st);
+size_t prefix_workspace_bytes(const carekv_prefix_t& p, int rows, int heads);
+cudaError_t launch_prefix(const carekv_prefix_t& p, const void* q, int64_t q_row, int64_t q_head, int rows, int heads,
+                          float scale, const int32_t* lengths, const void* tail, const float* tail_lse, void* out,
+                          float* lse, void* ws, cudaStream_t st);
 struct DecodeArgs;
 template <int QN>
 cudaError_t launch_decode_generic(DecodeArgs& a, cudaStream_t st, int n_bh);

@@ -1,0 +1,126 @@
+"""Attention of a whole batch over one shared prompt prefix.
+
+Sequences that start with the same prompt hold its K / V once, at full
+precision, instead of once per sequence in the packed arena: its bytes are
+shared by the batch, so quantizing them would save little, and every tile is
+read once per step for all sequences.  The sequences' own tokens stay in the
+arena; ``DecodeEngine.attend(..., prefix=...)`` merges both.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from ._tensors import dtype_code, need_cuda, need_like, on_device, rows_of, stream
+
+
+def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = None,
+                     lengths: Optional[Tensor] = None, tail: Optional[Tuple[Tensor, Tensor]] = None,
+                     out: Optional[Tensor] = None, return_lse: bool = False) -> Union[Tensor, Tuple[Tensor, Tensor]]:
+    """softmax(scale q K^T) V of every row over the prefix, merged with the
+    rows' own attention state.
+
+    q [n, Hq, D]; k, v [Hkv, N, D] (Hq a multiple of Hkv; any strides with
+    unit channel stride; N may be 0); scale defaults to 1 / sqrt(D).  lengths
+    [n] int32: row r sees the prefix tokens below lengths[r] (clamped to
+    0..N).  tail = (o [n, Hq, D], lse [n, Hq] fp32): attention output and
+    natural log-sum-exp of the row's own tokens, -inf where it has none.
+    Returns [n, Hq, D] in q's dtype, with return_lse also the merged
+    log-sum-exp [n, Hq] fp32; a row that sees nothing gives 0 and -inf.
+    Values of a token that any row sees must be finite for every row.
+    """
+    need_cuda(q, "prefix_attention q")
+    p = _lib.Prefix()
+    p.dtype = dtype_code(q, "prefix_attention q")
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"prefix_attention: expected q [n, Hq, D] and k, v [Hkv, N, D], got {tuple(q.shape)} and "
+                         f"{tuple(k.shape)}")
+    n, hq, d = q.shape
+    hkv, tokens, dk = k.shape
+    need_like(k, q, "prefix_attention k")
+    need_like(v, q, "prefix_attention v")
+    if dk != d or v.shape != k.shape:
+        raise ValueError(f"prefix_attention: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
+    if hkv < 1 or hq < 1 or hq % hkv:
+        raise ValueError(f"prefix_attention: {hq} query heads over {hkv} kv heads")
+    q, k, v = rows_of(q), rows_of(k), rows_of(v)
+    if lengths is not None:
+        if lengths.device != q.device or lengths.dtype is not torch.int32 or tuple(lengths.shape) != (n,):
+            raise ValueError(f"prefix_attention lengths: expected int32 [{n}] on {q.device}")
+        lengths = lengths.contiguous()
+    tail_o = tail_lse = None
+    if tail is not None:
+        tail_o, tail_lse = tail
+        need_like(tail_o, q, "prefix_attention tail output")
+        if tail_o.shape != q.shape or tail_lse.shape != q.shape[:2] or tail_lse.dtype is not torch.float32 \
+                or tail_lse.device != q.device:
+            raise ValueError("prefix_attention tail: expected (output like q, fp32 log-sum-exp [n, Hq])")
+        tail_o, tail_lse = tail_o.contiguous(), tail_lse.contiguous()
+    if out is None:
+        out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+    else:
+        need_like(out, q, "prefix_attention out")
+        if out.shape != q.shape or not out.is_contiguous():
+            raise ValueError(f"prefix_attention out: expected a contiguous tensor of shape {tuple(q.shape)}")
+    lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
+    p.k, p.v = k.data_ptr(), v.data_ptr()
+    ks, vs = k.stride(), v.stride()
+    p.k_stride[0], p.k_stride[1] = ks[0], ks[1]
+    p.v_stride[0], p.v_stride[1] = vs[0], vs[1]
+    p.num_kv_heads, p.tokens, p.head_dim = hkv, tokens, d
+    lib = _lib.lib()
+    need = ctypes.c_size_t(0)
+    qs = q.stride()
+    with on_device(q):
+        _lib.check(lib.carekv_prefix_workspace_bytes(ctypes.byref(p), n, hq, ctypes.byref(need)),
+                   "carekv_prefix_workspace_bytes")
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        _lib.check(lib.carekv_prefix_attention(
+            ctypes.byref(p), q.data_ptr(), qs[0], qs[1], n, hq, 1.0 / math.sqrt(d) if scale is None else scale,
+            None if lengths is None else lengths.data_ptr(), None if tail_o is None else tail_o.data_ptr(),
+            None if tail_lse is None else tail_lse.data_ptr(), out.data_ptr(),
+            None if lse is None else lse.data_ptr(), ws.data_ptr(), need.value, stream(q)),
+            "carekv_prefix_attention")
+    return (out, lse) if return_lse else out
+
+
+class SharedPrefix:
+    """K / V of one prompt prefix for every layer, post-RoPE at positions
+    0 .. tokens - 1, shared by all sequences of a cache."""
+
+    def __init__(self, num_layers: int):
+        self._kv = [None] * num_layers
+
+    def set(self, layer: int, k: Tensor, v: Tensor):
+        """k, v [Hkv, N, D] of one layer."""
+        if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError(f"SharedPrefix: k {tuple(k.shape)} and v {tuple(v.shape)} must match")
+        n = self.tokens
+        if n is not None and k.shape[1] != n:
+            raise ValueError(f"SharedPrefix: layer {layer} holds {k.shape[1]} tokens, the others {n}")
+        self._kv[layer] = (k.contiguous(), v.contiguous())
+
+    @property
+    def tokens(self) -> Optional[int]:
+        """Tokens of the prefix (None before any layer is set)."""
+        return next((kv[0].shape[1] for kv in self._kv if kv is not None), None)
+
+    def layer(self, layer: int) -> Tuple[Tensor, Tensor]:
+        kv = self._kv[layer]
+        if kv is None:
+            raise ValueError(f"SharedPrefix: layer {layer} has not been set")
+        return kv
+
+    def memory_bytes(self) -> int:
+        return sum(2 * kv[0].numel() * kv[0].element_size() for kv in self._kv if kv is not None)
+
+    def attend(self, layer: int, q: Tensor, **kw):
+        """prefix_attention of q [n, Hq, D] over this layer's prefix."""
+        k, v = self.layer(layer)
+        return prefix_attention(q, k, v, **kw)

@@ -1,0 +1,196 @@
+"""Rotary positions on the GPU: interleaved or half layout, all or part of the
+head, plain or scaled for contexts longer than the trained one.
+
+The reference rotates q and k with transformers' apply_rotary_pos_emb
+(layer.py:66) from cos / sin tables made on the host side of every step.
+Here a step hands over integer positions; frequencies are kept as 64-bit
+fractions of a turn, so a position's phase is one exact integer product and
+far positions lose no accuracy.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from ._tensors import dtype_code, need_cuda, need_like, on_device, rows_of, stream
+
+LAYOUTS = ("half", "interleaved")
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                       original_max_position: Optional[int] = None, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                       device=None) -> Tuple[Tensor, float]:
+    """(freq, attention_factor) of rotary_dim / 2 pairs: freq int64, pair i's
+    turns per position times 2^64; theta_i = base^(-2i / rotary_dim), scaled by
+
+    * "linear": theta / factor (positions squeezed into the trained range);
+    * "ntk": base grows to base * factor^(rd / (rd - 2)), so the slowest pair
+      is squeezed by `factor` and the fastest keeps its pace;
+    * "yarn": pairs that turn more than beta_fast times within
+      original_max_position keep theta, those below beta_slow turns get
+      theta / factor, with a linear ramp over the pairs between; rows are
+      scaled by 0.1 ln(factor) + 1.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if scaling not in ("none", "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling={scaling}: none, linear, ntk or yarn")
+    if not base > 1.0 or not factor >= 1.0:
+        raise ValueError(f"base={base} must be above 1 and factor={factor} at least 1")
+    if scaling == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("ntk scaling needs at least two pairs")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    theta = base ** (-2.0 * i / rotary_dim)
+    attention_factor = 1.0
+    if scaling == "linear":
+        theta = theta / factor
+    elif scaling == "yarn":
+        if not original_max_position or original_max_position < 1:
+            raise ValueError("yarn scaling needs original_max_position")
+
+        def pair_of(turns):   # the (fractional) pair that turns `turns` times over the trained range
+            return rotary_dim * math.log(original_max_position / (turns * 2 * math.pi)) / (2 * math.log(base))
+        lo = max(math.floor(pair_of(beta_fast)), 0)
+        hi = min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
+        ramp = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        theta = theta / factor * ramp + theta * (1 - ramp)
+        attention_factor = 0.1 * math.log(factor) + 1.0
+    turns = [round(t / (2 * math.pi) * 2.0 ** 64) for t in theta.tolist()]
+    return torch.tensor(turns, dtype=torch.int64, device=device), attention_factor
+
+
+def apply_rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, freq: Tensor, layout: str = "half",
+                 attention_factor: float = 1.0, inverse: bool = False,
+                 out: Optional[Tuple[Tensor, Optional[Tensor]]] = None) -> Tuple[Tensor, Optional[Tensor]]:
+    """Turn the first 2 * len(freq) channels of every row of q and k.
+
+    q [n, Hq, D] and k [n, Hkv, D] with positions [n], or q [B, T, Hq, D] and
+    k [B, T, Hkv, D] with positions [B, T] or [T]; any strides (transposed
+    views are read in place), positions int32 or int64 of any sign, k may be
+    None.  inverse turns back: it maps gradients of the results to gradients
+    of the inputs, which is also what autograd gets.  out = (q_out, k_out):
+    tensors of the same shapes to write to (any strides with unit channel
+    stride, apart from the inputs), new contiguous ones otherwise.
+    """
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if out is not None:
+            raise RuntimeError("apply_rotary: out= does not take part in autograd")
+        return _Turn.apply(q, k, positions, freq, layout, attention_factor, inverse)
+    return _turn(q, k, positions, freq, layout, attention_factor, inverse, out)
+
+
+class _Turn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, freq, layout, attention_factor, inverse):
+        ctx.args = (positions, freq, layout, attention_factor, not inverse)
+        ctx.shapes = (q.shape, None if k is None else k.shape)
+        return _turn(q, k, positions, freq, layout, attention_factor, inverse, None)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        qs, ks = ctx.shapes
+        like = dq if dq is not None else dk
+        if dq is None:
+            dq = like.new_zeros(qs)
+        if dk is None and ks is not None:
+            dk = like.new_zeros(ks)
+        return (*_turn(dq, dk, *ctx.args, None), None, None, None, None, None)
+
+
+def _fill(r: "_lib.Rows", x: Tensor, y: Tensor):
+    r.in_, r.out, r.heads = x.data_ptr(), y.data_ptr(), x.shape[-2]
+    si, so = x.stride(), y.stride()
+    if x.dim() == 4:
+        r.in_stride[0], r.in_stride[1], r.in_stride[2] = si[0], si[1], si[2]
+        r.out_stride[0], r.out_stride[1], r.out_stride[2] = so[0], so[1], so[2]
+    else:
+        r.in_stride[1], r.in_stride[2] = si[0], si[1]
+        r.out_stride[1], r.out_stride[2] = so[0], so[1]
+
+
+def _turn(q, k, positions, freq, layout, attention_factor, inverse, out):
+    need_cuda(q, "apply_rotary q")
+    a = _lib.Rotary()
+    a.dtype = dtype_code(q, "apply_rotary q")
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout={layout}: half or interleaved")
+    shape = q.shape
+    if q.dim() not in (3, 4):
+        raise ValueError(f"apply_rotary q: expected [n, H, D] or [B, T, H, D], got {tuple(shape)}")
+    lead, D = shape[:-2], shape[-1]
+    if k is not None:
+        need_like(k, q, "apply_rotary k")
+        if k.shape[:-2] != lead or k.shape[-1] != D or k.dim() != q.dim():
+            raise ValueError(f"apply_rotary k: {tuple(k.shape)} does not match q {tuple(shape)}")
+    if positions.device != q.device or freq.device != q.device:
+        raise RuntimeError(f"apply_rotary: positions and freq belong on {q.device}")
+    if positions.dtype is torch.int64:
+        a.position_bytes = 8
+    elif positions.dtype is torch.int32:
+        a.position_bytes = 4
+    else:
+        raise ValueError(f"apply_rotary positions: int32 or int64, got {positions.dtype}")
+    if positions.shape != lead and (len(lead) == 1 or positions.shape != lead[1:]):
+        raise ValueError(f"apply_rotary positions: {tuple(positions.shape)} does not match {tuple(lead)}")
+    if freq.dtype is not torch.int64 or freq.dim() != 1 or not freq.is_contiguous():
+        raise ValueError("apply_rotary freq: a contiguous int64 vector (rotary_frequencies)")
+    pairs = freq.shape[0]
+    if not 0 < 2 * pairs <= D:
+        raise ValueError(f"apply_rotary: {2 * pairs} rotary channels do not fit a head of {D}")
+    q = rows_of(q)
+    k = None if k is None else rows_of(k)
+    if out is None:
+        yq = torch.empty(shape, dtype=q.dtype, device=q.device)
+        yk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    else:
+        yq, yk = out
+        for x, y, what in ((q, yq, "q"), (k, yk, "k")):
+            if (x is None) != (y is None):
+                raise ValueError(f"apply_rotary out: one tensor for each of q and k ({what})")
+            if x is None:
+                continue
+            need_like(y, q, f"apply_rotary out {what}")
+            if y.shape != x.shape or (y.stride(-1) != 1 and D > 1):
+                raise ValueError(f"apply_rotary out {what}: expected shape {tuple(x.shape)} with unit channel stride")
+            held = y.untyped_storage().data_ptr()
+            if held == q.untyped_storage().data_ptr() or (k is not None and held == k.untyped_storage().data_ptr()):
+                raise ValueError("apply_rotary out: must not share storage with q or k")
+    if q.dim() == 4:
+        a.batch, a.tokens = lead
+    else:
+        a.batch, a.tokens = 1, lead[0]
+    sp = positions.stride()
+    a.position_stride[1] = sp[-1]
+    a.position_stride[0] = sp[0] if len(sp) == 2 else 0
+    a.positions, a.freq = positions.data_ptr(), freq.data_ptr()
+    a.head_dim, a.rotary_dim = D, 2 * pairs
+    a.interleaved, a.inverse, a.factor = layout == "interleaved", bool(inverse), attention_factor
+    _fill(a.q, q, yq)
+    if k is not None:
+        _fill(a.k, k, yk)
+    with on_device(q):
+        _lib.check(_lib.lib().carekv_rotary(ctypes.byref(a), stream(q)), "carekv_rotary")
+    return yq, yk
+
+
+class RotaryEmbedding:
+    """Frequencies and layout of a model's rotary positions, kept on the device."""
+
+    def __init__(self, rotary_dim: int, base: float = 10000.0, layout: str = "half", scaling: str = "none",
+                 factor: float = 1.0, original_max_position: Optional[int] = None, device="cuda"):
+        if layout not in LAYOUTS:
+            raise ValueError(f"layout={layout}: half or interleaved")
+        self.layout = layout
+        self.freq, self.attention_factor = rotary_frequencies(
+            rotary_dim, base, scaling, factor, original_max_position, device=device)
+
+    def __call__(self, q: Tensor, k: Optional[Tensor], positions: Tensor, inverse: bool = False, out=None):
+        return apply_rotary(q, k, positions, self.freq, self.layout, self.attention_factor, inverse, out)

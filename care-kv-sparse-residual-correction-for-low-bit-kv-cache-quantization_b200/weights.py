@@ -1,0 +1,110 @@
+"""4-bit weights with group scales for the projections of a decode step.
+
+The codes and scales are the package quantizer's (``quantize`` with 4 bits,
+``pack_int4_2d``); a PackedWeight holds them once more in the order in which
+the product kernel's lanes read them, made when a model is loaded.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from ._tensors import dtype_code, need_cuda, need_like, on_device, stream
+from .quantizer import QuantConfig, pack_codes_2d, quantize
+
+# rows up to which matmul multiplies from the codes (PackedWeight.matmul)
+MATVEC_ROWS = 64
+
+
+class PackedWeight:
+    """Weight [N, K] as 4-bit codes -8..7 times one scale per `group_size`
+    channels of a row.  packed [N, K/2]: rows of ``pack_int4_2d``; scale
+    [N, K/group_size] in the activations' dtype."""
+
+    def __init__(self, packed: Tensor, scale: Tensor, group_size: int):
+        need_cuda(packed, "PackedWeight packed")
+        need_cuda(scale, "PackedWeight scale")
+        if packed.dtype not in (torch.uint8, torch.int8) or packed.dim() != 2:
+            raise ValueError(f"PackedWeight packed: expected a 2-d byte tensor, got {packed.dtype} "
+                             f"{tuple(packed.shape)}")
+        if scale.device != packed.device:
+            raise RuntimeError(f"PackedWeight scale: expected a tensor on {packed.device}, got {scale.device}")
+        n, k = packed.shape[0], 2 * packed.shape[1]
+        if group_size < 1 or k % group_size or tuple(scale.shape) != (n, k // group_size):
+            raise ValueError(f"PackedWeight: scale {tuple(scale.shape)} does not fit {n} rows of {k} channels in "
+                             f"groups of {group_size}")
+        packed, scale = packed.contiguous(), scale.contiguous()
+        self.shape = (n, k)
+        self.group_size = group_size
+        self.dtype = scale.dtype
+        self.device = packed.device
+        self.c = _lib.W4()
+        self.c.n, self.c.k, self.c.group_size = n, k, group_size
+        self.c.dtype = dtype_code(scale, "PackedWeight scale")
+        sizes = (ctypes.c_size_t * 2)()
+        lib = _lib.lib()
+        _lib.check(lib.carekv_w4_layout(ctypes.byref(self.c), sizes), "carekv_w4_layout")
+        self.codes = torch.empty(sizes[0], dtype=torch.uint8, device=packed.device)
+        self.scales = torch.empty(sizes[1], dtype=torch.uint8, device=packed.device)
+        self.c.codes, self.c.scales = self.codes.data_ptr(), self.scales.data_ptr()
+        with on_device(packed):
+            _lib.check(lib.carekv_w4_pack(ctypes.byref(self.c), packed.data_ptr(), scale.data_ptr(), stream(packed)),
+                       "carekv_w4_pack")
+
+    @classmethod
+    def from_dense(cls, weight: Tensor, group_size: int = 32) -> "PackedWeight":
+        """Quantize a dense weight [N, K] with the package quantizer."""
+        codes, scale = quantize(weight, QuantConfig(bits=4, group_size=group_size))
+        return cls(pack_codes_2d(codes, 4), scale, group_size)
+
+    def memory_bytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def matvec(self, x: Tensor, out: Optional[Tensor] = None) -> Tensor:
+        """x [..., K] @ weight^T -> [..., N] in x's dtype (the scales' dtype),
+        read from the codes: made for the few rows of a decode step."""
+        n, k = self.shape
+        if x.device != self.device:
+            raise RuntimeError(f"matvec x: expected a tensor on {self.device}, got {x.device}")
+        if x.dtype is not self.dtype:
+            raise ValueError(f"matvec x: expected {self.dtype}, got {x.dtype}")
+        if x.shape[-1] != k:
+            raise ValueError(f"matvec x: expected [..., {k}], got {tuple(x.shape)}")
+        if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) < k or x.stride(0) % 8:
+            x2 = x.reshape(-1, k).contiguous()
+        else:
+            x2 = x
+        if x2.data_ptr() % 16:
+            x2 = x2.clone(memory_format=torch.contiguous_format)
+        shape = (*x.shape[:-1], n)
+        if out is None:
+            out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        else:
+            need_like(out, x, "matvec out")
+            if tuple(out.shape) != shape or not out.is_contiguous():
+                raise ValueError(f"matvec out: expected a contiguous tensor of shape {shape}")
+        with on_device(x):
+            _lib.check(_lib.lib().carekv_w4_matvec(ctypes.byref(self.c), x2.data_ptr(), max(x2.stride(0), k),
+                                                   x2.shape[0], out.data_ptr(), stream(x)), "carekv_w4_matvec")
+        return out
+
+    def dequantize(self) -> Tensor:
+        """The dense weight [N, K], codes * scale rounded to the scales' dtype."""
+        out = torch.empty(self.shape, dtype=self.dtype, device=self.device)
+        with on_device(out):
+            _lib.check(_lib.lib().carekv_w4_dequantize(ctypes.byref(self.c), out.data_ptr(), stream(out)),
+                       "carekv_w4_dequantize")
+        return out
+
+    def matmul(self, x: Tensor) -> Tensor:
+        """x [..., K] @ weight^T for any number of rows: from the codes up to
+        MATVEC_ROWS rows, above that (prompts) a dense product with the
+        dequantized weight."""
+        if x.numel() <= MATVEC_ROWS * self.shape[1]:
+            return self.matvec(x)
+        return x @ self.dequantize().t()

@@ -408,6 +408,92 @@ int carekv_prefill_correction(const carekv_config_t *cfg, const carekv_cache_t *
                               const float *sketch_proj, void *workspace, size_t workspace_bytes,
                               void *stream);
 
+/* ---- the rest of a decode step --------------------------------------------- */
+/* Rotary positions.  Pair i of a row at position p turns by p theta_i:
+ * (a, b) -> factor (a cos - b sin, b cos + a sin); inverse turns back (the
+ * gradient of the inputs from the gradient of the outputs).  Pairs are
+ * (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved; channels from
+ * rotary_dim on are copied.  freq[i] = theta_i / (2 pi) as a fraction of
+ * 2^64 (so the phase of any position is exact); positions are int32 or
+ * int64 (position_bytes 4 or 8), any sign.  Strides are in elements, the
+ * channel stride is 1; `in` and `out` must not overlap.  q or k may hold 0
+ * heads.  The reference applies transformers' apply_rotary_pos_emb
+ * (layer.py:66) with host-made cos / sin tables instead. */
+typedef struct carekv_rows {
+    const void *in;
+    void       *out;
+    int64_t     in_stride[3];    /* batch, token, head */
+    int64_t     out_stride[3];
+    int32_t     heads;
+} carekv_rows_t;
+typedef struct carekv_rotary {
+    carekv_rows_t  q, k;
+    const int64_t *freq;         /* [rotary_dim / 2] */
+    const void    *positions;
+    int64_t        position_stride[2];   /* batch, token */
+    int32_t        position_bytes;
+    int32_t        batch, tokens;
+    int32_t        head_dim;     /* 1 .. 256 */
+    int32_t        rotary_dim;   /* even, 2 .. head_dim */
+    int32_t        interleaved;
+    int32_t        inverse;
+    float          factor;
+    int32_t        dtype;
+} carekv_rotary_t;
+int carekv_rotary(const carekv_rotary_t *args, void *stream);
+
+/* 4-bit weights [n][k] with one scale per group of group_size channels (32,
+ * 64 or a multiple of 128 dividing k), held in the layout of the product
+ * kernels.  codes and scales are device buffers of the sizes that
+ * carekv_w4_layout gives, 16-byte aligned, filled once by carekv_w4_pack
+ * from packed rows [n][k / 2] (carekv_pack_codes, bits 4) and scales
+ * [n][k / group_size] in `dtype`.  No counterpart in the reference, whose
+ * projections stay in the model's dtype. */
+typedef struct carekv_w4 {
+    void   *codes;
+    void   *scales;
+    int32_t n, k;
+    int32_t group_size;
+    int32_t dtype;               /* of the scales, the activations and the result */
+} carekv_w4_t;
+int carekv_w4_layout(const carekv_w4_t *w, size_t sizes[2]);
+int carekv_w4_pack(const carekv_w4_t *w, const void *packed, const void *scale, void *stream);
+/* out [n][k] = codes * scales, each rounded to `dtype`. */
+int carekv_w4_dequantize(const carekv_w4_t *w, void *out, void *stream);
+/* out [rows][n] = x [rows][k] . weight^T, exact codes times activations in
+ * fp32 sums, scales applied to the groups' sums.  x rows start at multiples
+ * of x_stride elements (x 16-byte aligned, x_stride * element size a
+ * multiple of 16). */
+int carekv_w4_matvec(const carekv_w4_t *w, const void *x, int64_t x_stride, int32_t rows, void *out,
+                     void *stream);
+
+/* A prefix held once for all sequences: k, v [num_kv_heads][tokens][head_dim]
+ * with strides in elements (channel stride 1). */
+typedef struct carekv_prefix {
+    const void *k, *v;
+    int64_t     k_stride[2];     /* kv head, token */
+    int64_t     v_stride[2];
+    int32_t     num_kv_heads, tokens;
+    int32_t     head_dim;        /* 1 .. 256 */
+    int32_t     dtype;           /* of k, v, q, the own state and the result */
+} carekv_prefix_t;
+int carekv_prefix_workspace_bytes(const carekv_prefix_t *prefix, int32_t rows, int32_t num_heads, size_t *bytes);
+/* Attention of `rows` query rows q [rows][num_heads][head_dim] (strides in
+ * elements) over the prefix, the prefix read once for all rows.  Row r sees
+ * the tokens below lengths[r] (NULL: all; values are clamped to 0 ..
+ * tokens).  tail_out / tail_lse, both or neither: the attention state
+ * [rows][num_heads][head_dim] in dtype / [rows][num_heads] of the rows' own
+ * tokens (natural log of their sum of exponentials, -inf: none), merged into
+ * the result.  out [rows][num_heads][head_dim], lse [rows][num_heads] (may be
+ * NULL) the merged state; a row that sees no token at all gets 0 and -inf.
+ * Tokens that some rows see must be finite for the others too: a weight of 0
+ * times an infinity is NaN.  Tokens no row sees may hold anything.
+ * Workspace: carekv_prefix_workspace_bytes, 16-byte aligned. */
+int carekv_prefix_attention(const carekv_prefix_t *prefix, const void *q, int64_t q_row_stride,
+                            int64_t q_head_stride, int32_t rows, int32_t num_heads, float scale,
+                            const int32_t *lengths, const void *tail_out, const float *tail_lse, void *out,
+                            float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Copy the device error flag to the host and clear it (synchronizes the
  * stream).  Returns CAREKV_OK when no device check tripped. */
 int carekv_check_device_errors(const carekv_cache_t *cache, int32_t *flags_out, void *stream);

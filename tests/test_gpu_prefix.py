@@ -1,0 +1,255 @@
+"""Attention over a shared prefix against 64-bit softmax (GPU).
+
+Tolerance, per element: with d = head_dim 2^-24 scale sum |q| |k| the largest
+error of an fp32 score, a weight is off by a factor 1 +- (2 d + 4e-6), plus half
+an ulp of the 16-bit type where weights enter the matrix product in it; the
+result is rounded once: |error| <= half ulp |o| + (half ulp + 2 d + 4e-6) sum p |v|.
+The log-sum-exp is off by at most d + 4e-6 (1 + |lse|).
+"""
+
+import math
+
+import pytest
+import torch
+
+from conftest import load_pkg
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+HALF_ULP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+def pkg():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    return load_pkg()
+
+
+def reference(q, k, v, scale, lengths, tail):
+    """(o, sum p |v|, lse, d) in float64, shaped [n, Hq, ...]."""
+    n, hq, D = q.shape
+    hkv, N, _ = k.shape
+    g = hq // hkv
+    kd, vd = k.double().repeat_interleave(g, 0), v.double().repeat_interleave(g, 0)
+    qd = q.double().transpose(0, 1)
+    seen = torch.full((n,), N, device=q.device) if lengths is None else lengths.long().clamp(0, N)
+    top = int(seen.max()) if n else 0
+    kd, vd = kd[:, :top], vd[:, :top]
+    s = scale * qd @ kd.transpose(1, 2)                                   # [Hq, n, top]
+    hide = torch.arange(top, device=q.device) >= seen.unsqueeze(-1)
+    s = s.masked_fill(hide, -math.inf)
+    d = (D * 2.0 ** -24 * scale * (qd.abs() @ kd.abs().transpose(1, 2))).masked_fill(hide, 0.0)
+    d = d.amax(-1) if top else torch.zeros(hq, n, dtype=torch.float64, device=q.device)
+    lse = torch.logsumexp(s, -1) if top else torch.full((hq, n), -math.inf, dtype=torch.float64, device=q.device)
+    p = torch.exp(s - torch.where(lse > -math.inf, lse, 0.0).unsqueeze(-1))
+    o, size = p @ vd, p @ vd.abs()
+    o, size, lse, d = (x.transpose(0, 1) for x in (o, size, lse, d))
+    if tail is not None:
+        to, tl = tail[0].double(), tail[1].double()
+        both = torch.logaddexp(lse, tl)
+        ref = torch.where(both > -math.inf, both, 0.0)
+        a, b = torch.exp(lse - ref).unsqueeze(-1), torch.exp(tl - ref).unsqueeze(-1)
+        to = torch.where(b > 0, to, 0.0)
+        o, size, lse = a * o + b * to, a * size + b * to.abs(), both
+    return o, size, lse, d
+
+
+def check(got, lse, q, k, v, dtype, scale=None, lengths=None, tail=None):
+    scale = 1 / math.sqrt(q.shape[-1]) if scale is None else scale
+    o, size, ref_lse, d = reference(q, k, v, scale, lengths, tail)
+    h = HALF_ULP[dtype]
+    tol = h * o.abs() + (h + 2 * d.unsqueeze(-1) + 4e-6) * size + (2.0 ** -24 if dtype == "f16" else 1e-30)
+    err = (got.double() - o).abs()
+    assert got.dtype == q.dtype and bool((err <= tol).all()), float((err - tol).max())
+    some = ref_lse > -math.inf
+    assert torch.equal(lse > -math.inf, some)
+    off = (lse.double() - ref_lse)[some].abs()
+    assert bool((off <= (d + 4e-6 * (1 + ref_lse.abs()))[some]).all()), float(off.max())
+    assert bool((got[~some] == 0).all())
+
+
+def inputs(n, hq, hkv, D, N, dtype, seed=0, outliers=True):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randn(n, hq, D, device="cuda", generator=g)
+    k = torch.randn(hkv, N, D, device="cuda", generator=g)
+    if outliers:
+        k[..., : max(1, D // 32)] *= 8
+    v = torch.randn(hkv, N, D, device="cuda", generator=g)
+    return q.to(DT[dtype]), k.to(DT[dtype]), v.to(DT[dtype])
+
+
+def own_state(n, hq, D, dtype, seed=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    o = (0.3 * torch.randn(n, hq, D, device="cuda", generator=g)).to(DT[dtype])
+    lse = 3 + 4 * torch.randn(n, hq, device="cuda", generator=g)
+    lse[::3] = -math.inf
+    o[::3] = float("nan")     # a state of no tokens may hold anything
+    return o, lse
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,hq,hkv", [(1, 4, 4), (1, 8, 1), (3, 14, 2), (17, 8, 2), (33, 32, 4), (130, 3, 3),
+                                      (300, 8, 1)])
+def test_sizes(dtype, D, n, hq, hkv):
+    ck = pkg()
+    for N in (1, 2, 31, 64, 127, 128, 129, 255, 300, 513, 1100):
+        q, k, v = inputs(n, hq, hkv, D, N, dtype, N)
+        o, lse = ck.prefix_attention(q, k, v, return_lse=True)
+        check(o, lse, q, k, v, dtype)
+        tail = own_state(n, hq, D, dtype)
+        o, lse = ck.prefix_attention(q, k, v, tail=tail, return_lse=True, scale=0.05)
+        check(o, lse, q, k, v, dtype, scale=0.05, tail=tail)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,hq,hkv,D", [(40, 4, 2, 128), (200, 8, 2, 64), (9, 40, 40, 128), (300, 6, 2, 128)])
+def test_lengths(dtype, n, hq, hkv, D):
+    """Rows that see part of the prefix, none of it, or more than there is; what no row sees may hold NaN."""
+    ck = pkg()
+    for N, top in ((5, 3), (128, 128), (129, 128), (700, 389), (700, 700), (384, 257)):
+        q, k, v = inputs(n, hq, hkv, D, N, dtype, N)
+        g = torch.Generator(device="cuda").manual_seed(7)
+        lengths = torch.randint(0, top + 1, (n,), device="cuda", generator=g, dtype=torch.int32)
+        lengths[0], lengths[-1] = top, 0
+        if n > 4:
+            lengths[1] = -3
+        clean = (k.clone(), v.clone())
+        k[:, top:] = float("nan")
+        v[:, top:] = float("inf")
+        for tail in (None, own_state(n, hq, D, dtype)):
+            o, lse = ck.prefix_attention(q, k, v, lengths=lengths, tail=tail, return_lse=True)
+            check(o, lse, q, *clean, dtype, lengths=lengths, tail=tail)
+    # more than there is: the whole prefix
+    q, k, v = inputs(n, hq, hkv, D, 200, dtype)
+    o, lse = ck.prefix_attention(q, k, v, lengths=torch.full((n,), 10 ** 6, dtype=torch.int32, device="cuda"),
+                                 return_lse=True)
+    check(o, lse, q, k, v, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_no_tokens(dtype):
+    ck = pkg()
+    q, k, v = inputs(6, 4, 2, 64, 0, dtype)
+    o, lse = ck.prefix_attention(q, k, v, return_lse=True)
+    assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+    tail = own_state(6, 4, 64, dtype)
+    o, lse = ck.prefix_attention(q, k, v, tail=tail, return_lse=True)
+    check(o, lse, q, k, v, dtype, tail=tail)
+    q, k, v = inputs(5, 4, 2, 64, 300, dtype)
+    zero = torch.zeros(5, dtype=torch.int32, device="cuda")
+    o, lse = ck.prefix_attention(q, k, v, lengths=zero, return_lse=True)
+    assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+    assert ck.prefix_attention(q[:0], k, v).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_head_dims(dtype):
+    ck = pkg()
+    for D in (1, 24, 80, 96, 200, 256):
+        q, k, v = inputs(11, 6, 3, D, 150, dtype, D)
+        o, lse = ck.prefix_attention(q, k, v, return_lse=True)
+        check(o, lse, q, k, v, dtype)
+
+
+def test_strides_streams_and_out():
+    """Token-major K / V, views into a fused projection, another stream, a given output."""
+    ck = pkg()
+    for D in (64, 128):
+        n, hq, hkv, N = 21, 8, 2, 333
+        g = torch.Generator(device="cuda").manual_seed(D)
+        kv = torch.randn(N, 2 * hkv * D, device="cuda", generator=g).to(torch.bfloat16)
+        k = kv[:, : hkv * D].view(N, hkv, D).transpose(0, 1)
+        v = kv[:, hkv * D:].view(N, hkv, D).transpose(0, 1)
+        q = torch.randn(n, (hq + 3) * D, device="cuda", generator=g).to(torch.bfloat16)[:, D:(hq + 1) * D].view(n, hq, D)
+        o, lse = ck.prefix_attention(q, k, v, return_lse=True)
+        check(o, lse, q, k, v, "bf16")
+        out = torch.empty(n, hq, D, device="cuda", dtype=torch.bfloat16)
+        assert ck.prefix_attention(q, k, v, out=out) is out
+        assert torch.equal(out, o)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            other = ck.prefix_attention(q, k, v)
+        s.synchronize()
+        assert torch.equal(other, o)
+        # rows that start at odd elements, and channels that are not adjacent
+        odd = torch.randn(1 + hkv * N * D, device="cuda", generator=g).to(torch.bfloat16)[1:].view(hkv, N, D)
+        o, lse = ck.prefix_attention(q, odd, odd, return_lse=True)
+        check(o, lse, q, odd, odd, "bf16")
+        kt = torch.randn(hkv, D, N, device="cuda", generator=g).to(torch.bfloat16).transpose(1, 2)
+        qt = torch.randn(D, hq, n, device="cuda", generator=g).to(torch.bfloat16).permute(2, 1, 0)
+        o, lse = ck.prefix_attention(qt, kt, k, return_lse=True)
+        check(o, lse, qt, kt, k, "bf16")
+        # one kv head broadcast to several
+        kb = k[:1].expand(4, N, D)
+        o, lse = ck.prefix_attention(q, kb, kb, return_lse=True)
+        check(o, lse, q, kb, kb, "bf16")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_growing_maximum(dtype):
+    """Scores that rise (or fall) steadily by tens along the prefix: the running maximum moves at every tile."""
+    ck = pkg()
+    for D in (64, 128):
+        n, hq, hkv, N = 7, 8, 2, 1500
+        q, k, v = inputs(n, hq, hkv, D, N, dtype, 3, outliers=False)
+        q[..., 0] = 4.0
+        ramp = torch.linspace(-60, 60, N, device="cuda")
+        for r in (ramp, ramp.flip(0)):
+            k[..., 0] = r.to(k.dtype)
+            for lengths in (None, torch.arange(n, device="cuda", dtype=torch.int32) * 200):
+                o, lse = ck.prefix_attention(q, k, v, scale=1.0, lengths=lengths, return_lse=True)
+                check(o, lse, q, k, v, dtype, scale=1.0, lengths=lengths)
+
+
+def test_scores_of_the_types_lowest_value():
+    """Keys that push scores to the type's lowest value weigh nothing; a prefix of only such keys is an even mean."""
+    ck = pkg()
+    for dtype in ("f16", "bf16"):
+        n, hq, hkv, D, N = 5, 4, 2, 64, 200
+        q, k, v = inputs(n, hq, hkv, D, N, dtype, 5, outliers=False)
+        q[..., 0] = 1.0
+        k[..., 1:] = 0
+        k[..., 0] = 0
+        k[:, 50:150, 0] = torch.finfo(DT[dtype]).min
+        o, lse = ck.prefix_attention(q, k, v, scale=1.0, return_lse=True)
+        check(o, lse, q, k, v, dtype, scale=1.0)
+        k[..., 0] = torch.finfo(torch.float16).min
+        o, lse = ck.prefix_attention(q, k, v, scale=1.0, return_lse=True)
+        check(o, lse, q, k, v, dtype, scale=1.0)
+
+
+def test_shared_prefix_object():
+    ck = pkg()
+    q, k, v = inputs(4, 8, 2, 64, 100, "f16")
+    sp = ck.SharedPrefix(2)
+    assert sp.tokens is None
+    sp.set(0, k, v)
+    sp.set(1, v, k)
+    assert sp.tokens == 100 and sp.memory_bytes() == 4 * k.numel() * 2
+    assert torch.equal(sp.attend(1, q), ck.prefix_attention(q, v, k))
+    with pytest.raises(ValueError, match="layer 0 holds 90"):
+        sp.set(0, k[:, :90], v[:, :90])
+    with pytest.raises(ValueError, match="has not been set"):
+        ck.SharedPrefix(1).attend(0, q)
+
+
+def test_refusals():
+    ck = pkg()
+    q, k, v = inputs(4, 8, 2, 64, 100, "f16")
+    with pytest.raises(ValueError, match="query heads"):
+        ck.prefix_attention(q[:, :7], k, v)
+    with pytest.raises(ValueError, match="expected"):
+        ck.prefix_attention(q, k.float(), v)
+    with pytest.raises(ValueError, match="do not fit"):
+        ck.prefix_attention(q, k, v[:, :50])
+    with pytest.raises(ValueError, match="lengths"):
+        ck.prefix_attention(q, k, v, lengths=torch.ones(4, dtype=torch.int64, device="cuda"))
+    with pytest.raises(ValueError, match="tail"):
+        ck.prefix_attention(q, k, v, tail=(q, torch.zeros(4, 8, device="cuda").half()))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ck.prefix_attention(q.cpu(), k, v)
+    with pytest.raises(ck._lib.CareKVError, match="unsupported"):
+        big = torch.zeros(1, 1, 512, device="cuda")
+        ck.prefix_attention(big, big, big)

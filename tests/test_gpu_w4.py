@@ -1,0 +1,141 @@
+"""4-bit weight products against 64-bit sums (GPU).
+
+Tolerance: codes and activations enter exactly; what rounds is the fp32 sum
+of the K products (at most K 2^-24 sum |w| |x|, each partial sum once) and the
+result's own dtype (half an ulp).
+"""
+
+import pytest
+import torch
+
+from conftest import load_pkg
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+HALF_ULP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+def pkg():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    return load_pkg()
+
+
+def weight(n, k, group, dtype, seed=0):
+    """Random packed rows, scales, and the weight they stand for (float64)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(-8, 8, (n, k), device="cuda", generator=g)
+    scale = (0.01 + 0.1 * torch.rand(n, k // group, device="cuda", generator=g)).to(DT[dtype])
+    packed = ((codes[:, 0::2] & 15) | ((codes[:, 1::2] & 15) << 4)).to(torch.uint8)
+    return packed, scale, codes.double() * scale.double().repeat_interleave(group, 1)
+
+
+def check(got, x, w, dtype):
+    x = x.double().reshape(-1, w.shape[1])
+    ref, size = x @ w.T, x.abs() @ w.abs().T
+    tol = HALF_ULP[dtype] * ref.abs() + w.shape[1] * 2.0 ** -24 * size + (2.0 ** -24 if dtype == "f16" else 0.0)
+    err = (got.double().reshape(ref.shape) - ref).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,k,group", [(16, 128, 32), (1, 32, 32), (37, 96, 32), (64, 320, 64), (130, 1024, 128),
+                                       (250, 768, 256), (1000, 4096, 32), (33, 5632, 64)])
+def test_against_sums(dtype, n, k, group):
+    ck = pkg()
+    packed, scale, w = weight(n, k, group, dtype, n + k)
+    pw = ck.PackedWeight(packed, scale, group)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for m in (1, 2, 7, 8, 9, 16, 17, 32, 33, 64, 65, 130):
+        x = torch.randn(m, k, device="cuda", generator=g).to(DT[dtype])
+        y = pw.matvec(x)
+        assert y.shape == (m, n) and y.dtype == x.dtype
+        check(y, x, w, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_shapes_of_the_model_layers(dtype):
+    ck = pkg()
+    for n, k, group, m in ((4096, 4096, 32, 3), (2048, 5632, 64, 1), (5120, 13824, 64, 20), (14336, 4096, 128, 48)):
+        packed, scale, w = weight(n, k, group, dtype, n)
+        x = torch.randn(m, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(DT[dtype])
+        check(ck.PackedWeight(packed, scale, group).matvec(x), x, w, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_quantized_dense_weight(dtype):
+    """from_dense = the package quantizer's codes and scales; dequantize and matmul agree with them."""
+    ck = pkg()
+    g = torch.Generator(device="cuda").manual_seed(4)
+    dense = (torch.randn(72, 256, device="cuda", generator=g) / 16).to(DT[dtype])
+    pw = ck.PackedWeight.from_dense(dense, group_size=64)
+    codes, scale = ck.quantize(dense, ck.QuantConfig(bits=4, group_size=64))
+    w = codes.double() * scale.double().repeat_interleave(64, 1)
+    assert torch.equal(pw.dequantize(), (codes.float() * scale.float().repeat_interleave(64, 1)).to(DT[dtype]))
+    x = torch.randn(5, 256, device="cuda", generator=g).to(DT[dtype])
+    check(pw.matvec(x), x, w, dtype)
+    assert torch.equal(pw.matmul(x), pw.matvec(x))
+    big = torch.randn(200, 256, device="cuda", generator=g).to(DT[dtype])
+    # above the row limit the weight itself is rounded to the dtype: its half ulp joins
+    ref, size = big.double() @ w.T, big.double().abs() @ w.abs().T
+    tol = HALF_ULP[dtype] * (ref.abs() + size) + 256 * 2.0 ** -24 * size
+    assert bool(((pw.matmul(big).double() - ref).abs() <= tol).all())
+
+
+def test_infinite_and_nan_activations_stay_in_their_row():
+    ck = pkg()
+    for dtype in DT:
+        packed, scale, w = weight(40, 160, 32, dtype, 9)
+        x = torch.randn(4, 160, device="cuda").to(DT[dtype])
+        x[1, 5] = float("nan")
+        x[2, 7] = float("inf")
+        y = ck.PackedWeight(packed, scale, 32).matvec(x)
+        assert bool(y[1].isnan().all())
+        c = w[:, 7]
+        assert bool(y[2][c > 0].eq(float("inf")).all()) and bool(y[2][c < 0].eq(float("-inf")).all())
+        assert bool(y[2][c == 0].isnan().all())
+        check(y[0::3], x[0::3], w, dtype)
+
+
+def test_strides_streams_and_out():
+    ck = pkg()
+    packed, scale, w = weight(50, 256, 32, "f16", 11)
+    pw = ck.PackedWeight(packed, scale, 32)
+    wide = torch.randn(6, 512, device="cuda").half()
+    for x in (wide[:, 256:], wide[:, :256], wide[::2, 3:259], wide[:, ::2], wide.view(2, 3, 512)[..., :256],
+              wide[:1, :256].expand(3, 256), wide[0, :256]):
+        y = pw.matvec(x)
+        assert y.shape == (*x.shape[:-1], 50)
+        check(y, x, w, "f16")
+    assert pw.matvec(wide[:0, :256]).shape == (0, 50)
+    out = torch.empty(6, 50, device="cuda", dtype=torch.float16)
+    assert pw.matvec(wide[:, :256], out=out) is out
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = pw.matvec(wide[:, :256])
+    s.synchronize()
+    assert torch.equal(other, out)
+
+
+def test_refusals():
+    ck = pkg()
+    packed, scale, _ = weight(16, 128, 32, "f16")
+    pw = ck.PackedWeight(packed, scale, 32)
+    with pytest.raises(ValueError, match="expected"):
+        pw.matvec(torch.randn(2, 128, device="cuda"))
+    with pytest.raises(ValueError, match="expected"):
+        pw.matvec(torch.randn(2, 64, device="cuda").half())
+    with pytest.raises(RuntimeError):
+        pw.matvec(torch.randn(2, 128).half())
+    with pytest.raises(ValueError, match="out"):
+        pw.matvec(torch.randn(2, 128, device="cuda").half(), out=torch.empty(2, 17, device="cuda").half())
+    with pytest.raises(ValueError, match="scale"):
+        ck.PackedWeight(packed, scale[:, :3], 32)
+    with pytest.raises(ValueError, match="byte"):
+        ck.PackedWeight(packed.float(), scale, 32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ck.PackedWeight(packed.cpu(), scale, 32)
+    p16, s16, _ = weight(16, 128, 16, "f16")
+    with pytest.raises(ck._lib.CareKVError, match="unsupported"):
+        ck.PackedWeight(p16, s16, 16)
