@@ -487,6 +487,7 @@ int carekv_prefix_attention(const carekv_prefix_t* p, const void* q, int64_t q_r
   CHECK(validate_prefix(p, rows, heads));
   if (rows == 0) return CAREKV_OK;
   if (!q || !out || (p->tokens > 0 && (!p->k || !p->v))) return CAREKV_ERR_INVALID_ARG;
+  if (!(scale > 0.f)) return CAREKV_ERR_INVALID_ARG;
   if ((tail_out == nullptr) != (tail_lse == nullptr)) return CAREKV_ERR_INVALID_ARG;
   const size_t need = prefix_workspace_bytes(*p, rows, heads);
   if (need > 0 && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15))) return CAREKV_ERR_INVALID_ARG;

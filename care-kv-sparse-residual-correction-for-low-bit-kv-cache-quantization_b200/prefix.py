@@ -27,7 +27,7 @@ def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = N
     rows' own attention state.
 
     q [n, Hq, D]; k, v [Hkv, N, D] (Hq a multiple of Hkv; any strides with
-    unit channel stride; N may be 0); scale defaults to 1 / sqrt(D).  lengths
+    unit channel stride; N may be 0); scale > 0 defaults to 1 / sqrt(D).  lengths
     [n] int32: row r sees the prefix tokens below lengths[r] (clamped to
     0..N).  tail = (o [n, Hq, D], lse [n, Hq] fp32): attention output and
     natural log-sum-exp of the row's own tokens, -inf where it has none.

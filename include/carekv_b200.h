@@ -479,7 +479,7 @@ typedef struct carekv_prefix {
 } carekv_prefix_t;
 int carekv_prefix_workspace_bytes(const carekv_prefix_t *prefix, int32_t rows, int32_t num_heads, size_t *bytes);
 /* Attention of `rows` query rows q [rows][num_heads][head_dim] (strides in
- * elements) over the prefix, the prefix read once for all rows.  Row r sees
+ * elements) over the prefix, the prefix read once for all rows; scale > 0.  Row r sees
  * the tokens below lengths[r] (NULL: all; values are clamped to 0 ..
  * tokens).  tail_out / tail_lse, both or neither: the attention state
  * [rows][num_heads][head_dim] in dtype / [rows][num_heads] of the rows' own
