@@ -6,6 +6,7 @@ every entry point raises; there is no CPU fallback.
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libcarekv_b200.so")
@@ -82,6 +83,12 @@ class Rotary(ctypes.Structure):
                 ("interleaved", i32), ("inverse", i32), ("factor", f32), ("dtype", i32)]
 
 
+# The same bytes as a Rotary / Prefix structure, packed in one call: setting
+# three dozen ctypes fields one by one takes longer than the launch.
+ROTARY_PACK = struct.Struct("@PP6qi4xPP6qi4xPP2q7ifi4x").pack
+PREFIX_PACK = struct.Struct("@PP2q2q4i").pack
+
+
 class W4(ctypes.Structure):
     _fields_ = [("codes", vp), ("scales", vp), ("n", i32), ("k", i32), ("group_size", i32), ("dtype", i32)]
 
@@ -127,13 +134,13 @@ SIGNATURES = [
     ("carekv_decode_attention_shard", i32, [ctypes.POINTER(Config), ctypes.POINTER(Cache), i32, vp, vp, i32, i32,
                                             i32, i32, ctypes.POINTER(RouteParams), vp, vp, ctypes.c_size_t,
                                             ctypes.POINTER(Shard), vp]),
-    ("carekv_rotary", i32, [ctypes.POINTER(Rotary), vp]),
+    ("carekv_rotary", i32, [vp, vp]),   # carekv_rotary_t as packed bytes
     ("carekv_w4_layout", i32, [ctypes.POINTER(W4), ctypes.POINTER(ctypes.c_size_t)]),
     ("carekv_w4_pack", i32, [ctypes.POINTER(W4), vp, vp, vp]),
     ("carekv_w4_dequantize", i32, [ctypes.POINTER(W4), vp, vp]),
     ("carekv_w4_matvec", i32, [ctypes.POINTER(W4), vp, i64, i32, vp, vp]),
-    ("carekv_prefix_workspace_bytes", i32, [ctypes.POINTER(Prefix), i32, i32, ctypes.POINTER(ctypes.c_size_t)]),
-    ("carekv_prefix_attention", i32, [ctypes.POINTER(Prefix), vp, i64, i64, i32, i32, f32, vp, vp, vp, vp, vp, vp,
+    ("carekv_prefix_workspace_bytes", i32, [vp, i32, i32, ctypes.POINTER(ctypes.c_size_t)]),   # packed carekv_prefix_t
+    ("carekv_prefix_attention", i32, [vp, vp, i64, i64, i32, i32, f32, vp, vp, vp, vp, vp, vp,
                                       ctypes.c_size_t, vp]),
 ]
 NOALLOC_MAX_BYTES = 64 << 20

@@ -10,6 +10,7 @@ arena; ``DecodeEngine.attend(..., prefix=...)`` merges both.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Tuple, Union
 
@@ -17,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._tensors import dtype_code, need_cuda, need_like, on_device, rows_of, stream
+from ._tensors import dtype_code, need_cuda, need_like, new_rows, on_device, rows_of, stream
 
 
 def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = None,
@@ -36,8 +37,7 @@ def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = N
     Values of a token that any row sees must be finite for every row.
     """
     need_cuda(q, "prefix_attention q")
-    p = _lib.Prefix()
-    p.dtype = dtype_code(q, "prefix_attention q")
+    dt = dtype_code(q, "prefix_attention q")
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"prefix_attention: expected q [n, Hq, D] and k, v [Hkv, N, D], got {tuple(q.shape)} and "
                          f"{tuple(k.shape)}")
@@ -59,35 +59,37 @@ def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = N
         tail_o, tail_lse = tail
         need_like(tail_o, q, "prefix_attention tail output")
         if tail_o.shape != q.shape or tail_lse.shape != q.shape[:2] or tail_lse.dtype is not torch.float32 \
-                or tail_lse.device != q.device:
+                or tail_lse.get_device() != q.get_device():
             raise ValueError("prefix_attention tail: expected (output like q, fp32 log-sum-exp [n, Hq])")
         tail_o, tail_lse = tail_o.contiguous(), tail_lse.contiguous()
     if out is None:
-        out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+        out = new_rows(q)
     else:
         need_like(out, q, "prefix_attention out")
         if out.shape != q.shape or not out.is_contiguous():
             raise ValueError(f"prefix_attention out: expected a contiguous tensor of shape {tuple(q.shape)}")
-    lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
-    p.k, p.v = k.data_ptr(), v.data_ptr()
-    ks, vs = k.stride(), v.stride()
-    p.k_stride[0], p.k_stride[1] = ks[0], ks[1]
-    p.v_stride[0], p.v_stride[1] = vs[0], vs[1]
-    p.num_kv_heads, p.tokens, p.head_dim = hkv, tokens, d
-    lib = _lib.lib()
-    need = ctypes.c_size_t(0)
-    qs = q.stride()
+    lse = q.new_empty((n, hq), dtype=torch.float32) if return_lse else None
+    prefix = _lib.PREFIX_PACK(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), hkv,
+                              tokens, d, dt)
     with on_device(q):
-        _lib.check(lib.carekv_prefix_workspace_bytes(ctypes.byref(p), n, hq, ctypes.byref(need)),
-                   "carekv_prefix_workspace_bytes")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        _lib.check(lib.carekv_prefix_attention(
-            ctypes.byref(p), q.data_ptr(), qs[0], qs[1], n, hq, 1.0 / math.sqrt(d) if scale is None else scale,
+        need = _workspace_bytes(n, hq, hkv, tokens, d, dt, q.get_device())
+        ws = q.new_empty(need, dtype=torch.uint8)
+        status = _lib.lib().carekv_prefix_attention(
+            prefix, q.data_ptr(), q.stride(0), q.stride(1), n, hq, 1.0 / math.sqrt(d) if scale is None else scale,
             None if lengths is None else lengths.data_ptr(), None if tail_o is None else tail_o.data_ptr(),
             None if tail_lse is None else tail_lse.data_ptr(), out.data_ptr(),
-            None if lse is None else lse.data_ptr(), ws.data_ptr(), need.value, stream(q)),
-            "carekv_prefix_attention")
+            None if lse is None else lse.data_ptr(), ws.data_ptr(), need, stream(q))
+    if status:
+        _lib.check(status, "carekv_prefix_attention")
     return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(n, hq, hkv, tokens, d, dt, _device) -> int:
+    need = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().carekv_prefix_workspace_bytes(_lib.PREFIX_PACK(0, 0, 0, 0, 0, 0, hkv, tokens, d, dt), n, hq,
+                                                        ctypes.byref(need)), "carekv_prefix_workspace_bytes")
+    return need.value
 
 
 class SharedPrefix:

@@ -10,7 +10,6 @@ far positions lose no accuracy.
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional, Tuple
 
@@ -18,7 +17,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._tensors import dtype_code, need_cuda, need_like, on_device, rows_of, stream
+from ._tensors import dtype_code, need_cuda, need_like, new_rows, on_device, rows_of, stream
 
 LAYOUTS = ("half", "interleaved")
 
@@ -105,79 +104,85 @@ class _Turn(torch.autograd.Function):
         return (*_turn(dq, dk, *ctx.args, None), None, None, None, None, None)
 
 
-def _fill(r: "_lib.Rows", x: Tensor, y: Tensor):
-    r.in_, r.out, r.heads = x.data_ptr(), y.data_ptr(), x.shape[-2]
-    si, so = x.stride(), y.stride()
+_NO_ROWS = (0, 0, 0, 0, 0, 0, 0, 0, 0)   # no tensor, no heads
+
+
+def _rows(x: Tensor, y: Tensor):
+    """carekv_rows_t of a row tensor and its result."""
     if x.dim() == 4:
-        r.in_stride[0], r.in_stride[1], r.in_stride[2] = si[0], si[1], si[2]
-        r.out_stride[0], r.out_stride[1], r.out_stride[2] = so[0], so[1], so[2]
-    else:
-        r.in_stride[1], r.in_stride[2] = si[0], si[1]
-        r.out_stride[1], r.out_stride[2] = so[0], so[1]
+        b, t, h, _ = x.stride()
+        ob, ot, oh, _ = y.stride()
+        return x.data_ptr(), y.data_ptr(), b, t, h, ob, ot, oh, x.shape[2]
+    t, h, _ = x.stride()
+    ot, oh, _ = y.stride()
+    return x.data_ptr(), y.data_ptr(), 0, t, h, 0, ot, oh, x.shape[1]
+
+
+def _check_out(q, k, out):
+    yq, yk = out
+    for x, y, what in ((q, yq, "q"), (k, yk, "k")):
+        if (x is None) != (y is None):
+            raise ValueError(f"apply_rotary out: one tensor for each of q and k ({what})")
+        if x is None:
+            continue
+        need_like(y, q, f"apply_rotary out {what}")
+        if y.shape != x.shape or (y.stride(-1) != 1 and x.shape[-1] > 1):
+            raise ValueError(f"apply_rotary out {what}: expected shape {tuple(x.shape)} with unit channel stride")
+        held = y.untyped_storage().data_ptr()
+        if held == q.untyped_storage().data_ptr() or (k is not None and held == k.untyped_storage().data_ptr()):
+            raise ValueError("apply_rotary out: must not share storage with q or k")
+    return yq, yk
 
 
 def _turn(q, k, positions, freq, layout, attention_factor, inverse, out):
     need_cuda(q, "apply_rotary q")
-    a = _lib.Rotary()
-    a.dtype = dtype_code(q, "apply_rotary q")
+    dt = dtype_code(q, "apply_rotary q")
     if layout not in LAYOUTS:
         raise ValueError(f"layout={layout}: half or interleaved")
-    shape = q.shape
-    if q.dim() not in (3, 4):
+    shape, nd = q.shape, q.dim()
+    if nd != 3 and nd != 4:
         raise ValueError(f"apply_rotary q: expected [n, H, D] or [B, T, H, D], got {tuple(shape)}")
-    lead, D = shape[:-2], shape[-1]
+    D = shape[-1]
+    batch, tokens = (shape[0], shape[1]) if nd == 4 else (1, shape[0])
     if k is not None:
         need_like(k, q, "apply_rotary k")
-        if k.shape[:-2] != lead or k.shape[-1] != D or k.dim() != q.dim():
+        if k.dim() != nd or k.shape[:-2] != shape[:-2] or k.shape[-1] != D:
             raise ValueError(f"apply_rotary k: {tuple(k.shape)} does not match q {tuple(shape)}")
     if positions.device != q.device or freq.device != q.device:
         raise RuntimeError(f"apply_rotary: positions and freq belong on {q.device}")
     if positions.dtype is torch.int64:
-        a.position_bytes = 8
+        position_bytes = 8
     elif positions.dtype is torch.int32:
-        a.position_bytes = 4
+        position_bytes = 4
     else:
         raise ValueError(f"apply_rotary positions: int32 or int64, got {positions.dtype}")
-    if positions.shape != lead and (len(lead) == 1 or positions.shape != lead[1:]):
-        raise ValueError(f"apply_rotary positions: {tuple(positions.shape)} does not match {tuple(lead)}")
+    ps = positions.shape
+    if len(ps) == 2 and nd == 4 and ps[0] == batch and ps[1] == tokens:
+        sb, stok = positions.stride()
+    elif len(ps) == 1 and ps[0] == tokens:
+        sb, stok = 0, positions.stride(0)
+    else:
+        raise ValueError(f"apply_rotary positions: {tuple(ps)} does not match {tuple(shape[:-2])}")
     if freq.dtype is not torch.int64 or freq.dim() != 1 or not freq.is_contiguous():
         raise ValueError("apply_rotary freq: a contiguous int64 vector (rotary_frequencies)")
-    pairs = freq.shape[0]
-    if not 0 < 2 * pairs <= D:
-        raise ValueError(f"apply_rotary: {2 * pairs} rotary channels do not fit a head of {D}")
+    rd = 2 * freq.shape[0]
+    if not 0 < rd <= D:
+        raise ValueError(f"apply_rotary: {rd} rotary channels do not fit a head of {D}")
     q = rows_of(q)
-    k = None if k is None else rows_of(k)
-    if out is None:
-        yq = torch.empty(shape, dtype=q.dtype, device=q.device)
-        yk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    else:
-        yq, yk = out
-        for x, y, what in ((q, yq, "q"), (k, yk, "k")):
-            if (x is None) != (y is None):
-                raise ValueError(f"apply_rotary out: one tensor for each of q and k ({what})")
-            if x is None:
-                continue
-            need_like(y, q, f"apply_rotary out {what}")
-            if y.shape != x.shape or (y.stride(-1) != 1 and D > 1):
-                raise ValueError(f"apply_rotary out {what}: expected shape {tuple(x.shape)} with unit channel stride")
-            held = y.untyped_storage().data_ptr()
-            if held == q.untyped_storage().data_ptr() or (k is not None and held == k.untyped_storage().data_ptr()):
-                raise ValueError("apply_rotary out: must not share storage with q or k")
-    if q.dim() == 4:
-        a.batch, a.tokens = lead
-    else:
-        a.batch, a.tokens = 1, lead[0]
-    sp = positions.stride()
-    a.position_stride[1] = sp[-1]
-    a.position_stride[0] = sp[0] if len(sp) == 2 else 0
-    a.positions, a.freq = positions.data_ptr(), freq.data_ptr()
-    a.head_dim, a.rotary_dim = D, 2 * pairs
-    a.interleaved, a.inverse, a.factor = layout == "interleaved", bool(inverse), attention_factor
-    _fill(a.q, q, yq)
     if k is not None:
-        _fill(a.k, k, yk)
+        k = rows_of(k)
+    if out is not None:
+        yq, yk = _check_out(q, k, out)
+    else:
+        yq = new_rows(q)
+        yk = None if k is None else new_rows(k)
+    args = _lib.ROTARY_PACK(*_rows(q, yq), *(_NO_ROWS if k is None else _rows(k, yk)), freq.data_ptr(),
+                            positions.data_ptr(), sb, stok, position_bytes, batch, tokens, D, rd,
+                            layout == "interleaved", bool(inverse), attention_factor, dt)
     with on_device(q):
-        _lib.check(_lib.lib().carekv_rotary(ctypes.byref(a), stream(q)), "carekv_rotary")
+        status = _lib.lib().carekv_rotary(args, stream(q))
+    if status:
+        _lib.check(status, "carekv_rotary")
     return yq, yk
 
 

@@ -52,6 +52,7 @@ class PackedWeight:
         self.codes = torch.empty(sizes[0], dtype=torch.uint8, device=packed.device)
         self.scales = torch.empty(sizes[1], dtype=torch.uint8, device=packed.device)
         self.c.codes, self.c.scales = self.codes.data_ptr(), self.scales.data_ptr()
+        self._ref, self._index = ctypes.byref(self.c), packed.get_device()
         with on_device(packed):
             _lib.check(lib.carekv_w4_pack(ctypes.byref(self.c), packed.data_ptr(), scale.data_ptr(), stream(packed)),
                        "carekv_w4_pack")
@@ -69,28 +70,32 @@ class PackedWeight:
         """x [..., K] @ weight^T -> [..., N] in x's dtype (the scales' dtype),
         read from the codes: made for the few rows of a decode step."""
         n, k = self.shape
-        if x.device != self.device:
+        if x.get_device() != self._index:
             raise RuntimeError(f"matvec x: expected a tensor on {self.device}, got {x.device}")
         if x.dtype is not self.dtype:
             raise ValueError(f"matvec x: expected {self.dtype}, got {x.dtype}")
-        if x.shape[-1] != k:
-            raise ValueError(f"matvec x: expected [..., {k}], got {tuple(x.shape)}")
-        if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) < k or x.stride(0) % 8:
-            x2 = x.reshape(-1, k).contiguous()
-        else:
-            x2 = x
-        if x2.data_ptr() % 16:
-            x2 = x2.clone(memory_format=torch.contiguous_format)
-        shape = (*x.shape[:-1], n)
+        shape = x.shape
+        if not shape or shape[-1] != k:
+            raise ValueError(f"matvec x: expected [..., {k}], got {tuple(shape)}")
+        # rows the kernel can read in place: unit channel stride, every row
+        # on a 16-byte boundary
+        flat = x
+        if len(shape) != 2 or x.stride(1) != 1 or x.stride(0) < k or x.stride(0) % 8:
+            flat = x.reshape(-1, k).contiguous()
+        if flat.data_ptr() % 16:
+            flat = flat.clone(memory_format=torch.contiguous_format)
+        rows = flat.shape[0]
         if out is None:
-            out = torch.empty(shape, dtype=x.dtype, device=x.device)
+            out = x.new_empty((rows, n) if len(shape) == 2 else (*shape[:-1], n))
         else:
             need_like(out, x, "matvec out")
-            if tuple(out.shape) != shape or not out.is_contiguous():
-                raise ValueError(f"matvec out: expected a contiguous tensor of shape {shape}")
+            if tuple(out.shape) != (*shape[:-1], n) or not out.is_contiguous():
+                raise ValueError(f"matvec out: expected a contiguous tensor of shape {(*shape[:-1], n)}")
         with on_device(x):
-            _lib.check(_lib.lib().carekv_w4_matvec(ctypes.byref(self.c), x2.data_ptr(), max(x2.stride(0), k),
-                                                   x2.shape[0], out.data_ptr(), stream(x)), "carekv_w4_matvec")
+            status = _lib.lib().carekv_w4_matvec(self._ref, flat.data_ptr(), max(flat.stride(0), k), rows,
+                                                 out.data_ptr(), stream(x))
+        if status:
+            _lib.check(status, "carekv_w4_matvec")
         return out
 
     def dequantize(self) -> Tensor:
