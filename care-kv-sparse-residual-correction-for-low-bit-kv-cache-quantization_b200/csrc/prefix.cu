@@ -12,6 +12,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "launch.h"
 #include "tcgen05.cuh"
 
 namespace carekv {
@@ -20,19 +21,25 @@ namespace {
 constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // How the prefix is cut: a unit is one block of tokens for one tile of rows,
-// units are numbered tile by tile (tiles of kv head 0 first) and CTA c takes
-// units [start(c), start(c + 1)).  What a CTA has of a tile it does not hold
-// whole is a partial, in slot 2c if the CTA starts inside the tile (or at its
-// first unit), in slot 2c + 1 if the tile starts inside the CTA.
+// units are numbered tile by tile (tiles of kv head 0 first).  Every group of
+// `group` consecutive units is shared evenly by `per` CTAs; a group is one
+// tile, or all units.  What a CTA has of a tile it does not hold whole is a
+// partial, in slot 2c if the tile is the CTA's first, else in slot 2c + 1.
 struct Split {
   int tile_rows;    // rows of a kv head per tile
-  int block;        // tokens per unit
   int tiles;        // tiles per kv head
   int blocks;       // units per tile
-  int64_t units;
+  int units;
   int ctas;
-  __host__ __device__ int64_t start(int64_t c) const { return c * units / ctas; }
-  __host__ __device__ int cta_of(int64_t u) const { return static_cast<int>(((u + 1) * ctas - 1) / units); }
+  int group, per, base, rem;   // base, rem = group / per, group % per
+  __host__ __device__ int start(int c) const {
+    const int g = c / per, i = c - g * per;
+    return g * group + i * base + (i < rem ? i : rem);
+  }
+  __host__ __device__ int cta_of(int u) const {
+    const int g = u / group, v = u - g * group, cut = rem * (base + 1);
+    return g * per + (v < cut ? v / (base + 1) : rem + (v - cut) / base);
+  }
 };
 
 struct PrefixArgs {
@@ -147,7 +154,7 @@ struct TcLayout {
   static constexpr int kSlots = (224 * 1024 - kQ) / kSlot;       // 224 KB with Q
   static constexpr int kMl = kQ + kSlots * kSlot;                // float2 [2][128]
   static constexpr int kBar = kMl + 2 * kTcRows * 8;
-  static constexpr int kBars = 2 * kSlots + 8;
+  static constexpr int kBars = 2 * kSlots + 10;
   static constexpr int kBytes = kBar + kBars * 8 + 16;
 };
 
@@ -173,16 +180,15 @@ struct Segment {
 };
 
 // The part of a tile in [u, u_end); the whole warp calls it.
-__device__ __forceinline__ Segment segment_at(const PrefixArgs& a, int64_t u, int64_t u_begin, int64_t u_end,
-                                              int64_t* next) {
+__device__ __forceinline__ Segment segment_at(const PrefixArgs& a, int u, int u_begin, int u_end, int* next) {
   Segment s;
-  const int64_t tile = u / a.sp.blocks, tile0 = tile * a.sp.blocks;
-  const int64_t end = min(u_end, tile0 + a.sp.blocks);
+  const int tile = u / a.sp.blocks, tile0 = tile * a.sp.blocks;
+  const int end = min(u_end, tile0 + a.sp.blocks);
   *next = end;
-  s.kvh = static_cast<int>(tile / a.sp.tiles);
-  s.rho0 = static_cast<int>(tile - static_cast<int64_t>(s.kvh) * a.sp.tiles) * a.sp.tile_rows;
-  s.b0 = static_cast<int>(u - tile0);
-  s.nb = static_cast<int>(end - u);
+  s.kvh = tile / a.sp.tiles;
+  s.rho0 = (tile - s.kvh * a.sp.tiles) * a.sp.tile_rows;
+  s.b0 = u - tile0;
+  s.nb = end - u;
   s.slot = end - u == a.sp.blocks ? -1 : 2 * static_cast<int>(blockIdx.x) + (u == u_begin ? 0 : 1);
   s.top = a.p.tokens;
   if (a.lengths) {
@@ -200,6 +206,21 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// two fp32 operations per instruction
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*reinterpret_cast<uint64_t*>(&r))
+      : "l"(*reinterpret_cast<uint64_t*>(&x)), "l"(*reinterpret_cast<uint64_t*>(&y)), "l"(*reinterpret_cast<uint64_t*>(&z)));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(*reinterpret_cast<uint64_t*>(&r))
+      : "l"(*reinterpret_cast<uint64_t*>(&x)), "l"(*reinterpret_cast<uint64_t*>(&y)));
+  return r;
+}
 template <bool BF>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   if constexpr (BF) {
@@ -210,6 +231,14 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   }
 }
 
+// A whole 32-byte sector per lane: the rows of a warp lie apart, and two
+// 16-byte stores would each write half a sector.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 // The state of one row -- maximum m, weight sum l, C channels of the sums
 // from channel c0 on -- as a partial or, for a whole tile, the row's result.
 template <int D, int C, bool BF>
@@ -218,9 +247,13 @@ __device__ __forceinline__ void store_row(const PrefixArgs& a, const Segment& s,
   if (s.slot >= 0) {
     const int64_t at = static_cast<int64_t>(s.slot) * a.sp.tile_rows + tile_row;
     if (first) a.ml[at] = make_float2(m, l);
-    float4* d = reinterpret_cast<float4*>(a.po + at * D + c0);
 #pragma unroll
-    for (int i = 0; i < C / 4; ++i) d[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    for (int i = 0; i < C; i += 8) {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(o[i + j]);
+      store32(a.po + at * D + c0 + i, w);
+    }
     return;
   }
   const int64_t i = static_cast<int64_t>(rho / a.group) * a.heads + s.kvh * a.group + rho % a.group;
@@ -232,27 +265,25 @@ __device__ __forceinline__ void store_row(const PrefixArgs& a, const Segment& s,
   const float L = fmaf(wo, l, wt);
   const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
   if (first && a.lse) a.lse[i] = L > 0.f || L != L ? (top + log2f(L)) * kLn2 : -INFINITY;
-  uint4* d = reinterpret_cast<uint4*>(static_cast<char*>(a.out) + (i * D + c0) * 2);
+  char* d = static_cast<char*>(a.out) + (i * D + c0) * 2;
   const uint4* t = reinterpret_cast<const uint4*>(static_cast<const char*>(a.tail) + (i * D + c0) * 2);
 #pragma unroll
-  for (int k = 0; k < C / 8; ++k) {
-    float v[8];
+  for (int k = 0; k < C; k += 16) {
+    uint32_t w[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = wo * o[8 * k + j];
-    if (own) {
-      const uint4 x = t[k];
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    for (int g = 0; g < 2; ++g) {
+      const uint4 x = own ? t[k / 8 + g] : make_uint4(0, 0, 0, 0);
+      const uint32_t y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        const int c = k + 8 * g + 2 * j;
         float2 f;
-        if constexpr (BF) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
-        else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-        v[2 * j] = fmaf(wt, f.x, v[2 * j]);
-        v[2 * j + 1] = fmaf(wt, f.y, v[2 * j + 1]);
+        if constexpr (BF) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y[j]));
+        else f = __half22float2(*reinterpret_cast<const __half2*>(&y[j]));
+        w[4 * g + j] = pack16<BF>(fmaf(wt, f.x, wo * o[c]) * inv, fmaf(wt, f.y, wo * o[c + 1]) * inv);
       }
     }
-    d[k] = make_uint4(pack16<BF>(v[0] * inv, v[1] * inv), pack16<BF>(v[2] * inv, v[3] * inv),
-                      pack16<BF>(v[4] * inv, v[5] * inv), pack16<BF>(v[6] * inv, v[7] * inv));
+    store32(d + 2 * k, w);
   }
 }
 
@@ -264,42 +295,51 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
   using Ly = TcLayout<D, PAIR>;
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Ly::kBar);
-  uint64_t *full = bars, *empty = bars + Ly::kSlots, *s_full = bars + 2 * Ly::kSlots, *p_full = s_full + 2,
-           *o_full = s_full + 4, *q_full = s_full + 6, *done = s_full + 7;
+  // p_half / p_full: weights of the first / last 64 tokens of a block
+  uint64_t *full = bars, *empty = bars + Ly::kSlots, *s_full = bars + 2 * Ly::kSlots, *p_half = s_full + 2,
+           *p_full = s_full + 4, *o_full = s_full + 6, *q_full = s_full + 8, *done = s_full + 9;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Ly::kBars);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 9) tmem_alloc(tmem_slot, 512);
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < Ly::kSlots; ++i) {
-      mbar_init(full + i, 1);
-      mbar_init(empty + i, 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 4);
-      mbar_init(o_full + i, 1);
-    }
-    mbar_init(q_full, 256);
-    mbar_init(done, 1);
-    *dead = 0;
-    fence_mbar_init();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  // columns: S (and P) of stream s at 128 s, O at 256 + 128 s
-  const int64_t u_begin = a.sp.start(blockIdx.x), u_end = a.sp.start(blockIdx.x + 1);
+  const int u_begin = a.sp.start(blockIdx.x), u_end = a.sp.start(blockIdx.x + 1);
   bool ok = true;
 
   if (warp == 8) {
-    // ── loads, in the order in which the products use them ──
+    // ── loads, in the order in which the products use them; the first ones
+    // are on their way before the CTA has set up the rest ──
+    if (lane == 0) {
+      for (int i = 0; i < Ly::kSlots; ++i) {
+        mbar_init(full + i, 1);
+        mbar_init(empty + i, 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(s_full + i, 1);
+        mbar_init(p_half + i, 4);
+        mbar_init(p_full + i, 4);
+        mbar_init(o_full + i, 1);
+      }
+      mbar_init(q_full, 256);
+      mbar_init(done, 1);
+      *dead = 0;
+      fence_mbar_init();
+    }
+    __syncwarp();
     int cnt = 0;
+    bool synced = false;
+    auto sync_once = [&]() {
+      if (!synced) {
+        tc_fence_before();
+        __syncthreads();
+        synced = true;
+      }
+    };
     auto load = [&](const CUtensorMap* map, int z, int block) {
       const int slot = cnt % Ly::kSlots;
-      ok = ok && __all_sync(0xffffffffu, wait_or(empty + slot, ((cnt / Ly::kSlots) & 1) ^ 1, dead));
-      if (!ok) return;
+      if (cnt >= Ly::kSlots) {
+        sync_once();
+        ok = ok && __all_sync(0xffffffffu, wait_or(empty + slot, ((cnt / Ly::kSlots) & 1) ^ 1, dead));
+        if (!ok) return;
+      }
       if (lane == 0) {
         unsigned char* dst = smem + Ly::kQ + slot * Ly::kSlot;
         mbar_expect_tx(full + slot, Ly::kSlot);
@@ -309,7 +349,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
       }
       ++cnt;
     };
-    for (int64_t u = u_begin; u < u_end && ok;) {
+    for (int u = u_begin; u < u_end && ok;) {
       const Segment s = segment_at(a, u, u_begin, u_end, &u);
       const int zk = s.kvh * k_heads, zv = s.kvh * v_heads;
       if (s.nb > 0) load(&kmap, zk, s.b0);
@@ -320,51 +360,65 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
         if (n < s.nb) load(&kmap, zk, s.b0 + n);
       }
     }
+    sync_once();
     // a copy in flight must land before the CTA ends (all have when ok)
     if (!ok && lane == 0)
       for (int i = max(0, cnt - Ly::kSlots); i < cnt; ++i) mbar_wait(full + i % Ly::kSlots, (i / Ly::kSlots) & 1);
   } else if (warp == 9) {
     // ── products ──
+    tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;   // columns: S (and P) of stream s at 128 s, O at 256 + 128 s
     constexpr uint32_t kIdS = mma_idesc(kTcRows, kTcBlock, BF, false), kIdO = mma_idesc(kTcRows, D, BF, true);
-    const uint32_t base = smem_addr(smem);
+    const uint32_t base = smem_addr(smem), lead = elect_one();
+    // descriptors of the first Q and tile; others differ in the address field
+    // (16-byte units) alone
+    const uint64_t qd = smem_desc(base, 16, 1024), kd = smem_desc(base + Ly::kQ, 16, 1024),
+                   vd = smem_desc(base + Ly::kQ, kTcBlock * 128, 1024);
     int cnt = 0, seg = 0;
     uint32_t ph[2] = {0, 0};
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && __all_sync(0xffffffffu, wait_or(bar, parity, dead));
+    };
     // next tile in load order
     auto take = [&]() {
       const int slot = cnt % Ly::kSlots;
-      ok = ok && __all_sync(0xffffffffu, wait_or(full + slot, (cnt / Ly::kSlots) & 1, dead));
+      wait(full + slot, (cnt / Ly::kSlots) & 1);
       ++cnt;
       return slot;
     };
     auto scores = [&](int stream, int slot) {
-      if (!ok || lane != 0) return;
-      const uint32_t qa = base + (PAIR ? stream * (kTcRows * D * 2) : 0), ka = base + Ly::kQ + slot * Ly::kSlot;
+      if (!ok) return;
+      const uint64_t qa = qd + (PAIR ? stream * (kTcRows * D * 2 / 16) : 0), ka = kd + slot * (Ly::kSlot / 16);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = (k / 4) * (kTcRows * 128) + (k % 4) * 32;
-        mma_ss(tmem + 128 * stream, smem_desc(qa + off, 16, 1024), smem_desc(ka + off, 16, 1024), kIdS, k > 0);
+        const int off = ((k / 4) * (kTcRows * 128) + (k % 4) * 32) / 16;
+        mma_ss(tmem + 128 * stream, qa + off, ka + off, kIdS, k > 0, lead);
       }
-      mma_commit(s_full + stream);
+      mma_commit(s_full + stream, lead);
     };
-    auto sums = [&](int stream, int slot, int steps, bool acc) {
-      if (!ok || lane != 0) return;
-      const uint32_t va = base + Ly::kQ + slot * Ly::kSlot;
-      for (int k = 0; k < steps; ++k)
-        mma_ts(tmem + 256 + 128 * stream, tmem + 128 * stream + 8 * k,
-               smem_desc(va + k * (16 * 128), kTcBlock * 128, 1024), kIdO, acc || k > 0);
+    // O += P V for the tokens of half h, 16 a step
+    auto sums = [&](int stream, int slot, int h, int steps, bool acc) {
+      if (!ok) return;
+      const uint32_t o = tmem + 256 + 128 * stream, p = tmem + 128 * stream + 32 * h;
+      const uint64_t va = vd + slot * (Ly::kSlot / 16) + h * (64 * 128 / 16);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (4 * h + k < steps) mma_ts(o, p + 8 * k, va + k * (16 * 128 / 16), kIdO, acc || h > 0 || k > 0, lead);
     };
     auto release = [&](int slot) {
-      if (ok && lane == 0) mma_commit(empty + slot);
+      if (ok) mma_commit(empty + slot, lead);
     };
-    auto weights_ready = [&](int stream) {
-      ok = ok && __all_sync(0xffffffffu, wait_or(p_full + stream, ph[stream], dead));
-      ph[stream] ^= 1;
-      tc_fence_after();
+    auto finish = [&](int stream) {
+      if (ok) mma_commit(o_full + stream, lead);
     };
-    for (int64_t u = u_begin; u < u_end && ok;) {
+    for (int u = u_begin; u < u_end && ok;) {
       const Segment s = segment_at(a, u, u_begin, u_end, &u);
       if (s.nb == 0) continue;
-      ok = ok && __all_sync(0xffffffffu, wait_or(q_full, seg & 1, dead));
+      wait(q_full, seg & 1);
       ++seg;
       int ks = take();
       scores(0, ks);
@@ -381,104 +435,133 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
       }
       for (int b = 0; b < s.nb && ok; ++b) {
         const int seen = min(kTcBlock, s.top - (s.b0 + b) * kTcBlock), steps = (seen + 15) / 16;
-        const int first = PAIR ? 0 : b & 1;
-        weights_ready(first);
-        const int vs = take();
-        if (ok && lane == 0 && seen < 16 * steps && s.top < a.p.tokens) {
-          // tokens of the last step that no row sees: their weights are 0,
-          // and 0 times whatever they hold must be 0
-          unsigned char* v = smem + Ly::kQ + vs * Ly::kSlot;
-          for (int t = seen; t < 16 * steps; ++t)
-            for (int c = 0; c < D / 64; ++c)
-              for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<uint4*>(v + c * (kTcBlock * 128) + t * 128 + 16 * i) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async();
-        }
-        sums(first, vs, steps, PAIR ? b > 0 : b > 1);
-        if constexpr (PAIR) {
-          const bool more = b + 1 < s.nb;
-          if (more) {
-            ks = take();
-            scores(0, ks);
-          } else if (ok && lane == 0) {
-            mma_commit(o_full);
+        int vs = 0;
+#pragma unroll
+        for (int i = 0; i < (PAIR ? 2 : 1); ++i) {
+          const int stream = PAIR ? i : b & 1;
+          const bool acc = b > (PAIR ? 0 : 1);
+          wait(p_half + stream, ph[stream]);
+          if (i == 0) {
+            vs = take();
+            if (ok && seen < 16 * steps && s.top < a.p.tokens) {
+              // tokens of the last step that no row sees: their weights are
+              // 0, and 0 times whatever they hold must be 0
+              unsigned char* v = smem + Ly::kQ + vs * Ly::kSlot;
+              for (int j = lane; j < (16 * steps - seen) * (D / 8); j += 32) {
+                const int t = seen + j / (D / 8), c = j % (D / 8);
+                *reinterpret_cast<uint4*>(v + (c >> 3) * (kTcBlock * 128) + t * 128 + 16 * (c & 7)) = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async();
+              __syncwarp();
+            }
           }
-          weights_ready(1);
-          sums(1, vs, steps, b > 0);
-          release(vs);
-          if (more) {
-            scores(1, ks);
-            release(ks);
-          } else if (ok && lane == 0) {
-            mma_commit(o_full + 1);
-          }
-        } else {
-          release(vs);
-          if (b + 2 < s.nb) {
-            ks = take();
-            scores(first, ks);
-            release(ks);
-          } else if (ok && lane == 0) {
-            mma_commit(o_full + first);
+          tc_fence_after();
+          sums(stream, vs, 0, steps, acc);
+          wait(p_full + stream, ph[stream]);
+          ph[stream] ^= 1;
+          tc_fence_after();
+          sums(stream, vs, 1, steps, acc);
+          const int n = b + (PAIR ? 1 : 2);
+          if (!PAIR || i == 1) release(vs);
+          if (n < s.nb) {
+            if (!PAIR || i == 0) ks = take();
+            scores(stream, ks);
+            if (!PAIR || i == 1) release(ks);
+          } else {
+            finish(stream);
           }
         }
       }
     }
-    if (!ok && lane == 0) {   // nothing of ours may still run when TMEM is freed
-      mma_commit(done);
+    if (!ok) {   // nothing of ours may still run when TMEM is freed
+      mma_commit(done, lead);
       mbar_wait(done, 0);
     }
     __syncwarp();
   } else {
     // ── softmax: stream `st`, row `t` of its tile ──
     const int st = warp >> 2, t = threadIdx.x & 127;
-    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;   // TMEM lane 32 (warp % 4)
-    const uint32_t ts = tmem + 128 * st + lanes, to = tmem + 256 + 128 * st + lanes;
+    const int tile_row = PAIR ? st * kTcRows + t : t;
     const float bias = BF ? 0.f : 7.f;
     const int total = a.rows * a.group;
+    // a row's place: query row r, kv head group member h
+    int rho, r, h;
+    auto place = [&](const Segment& s) {
+      rho = s.rho0 + tile_row;
+      r = rho < total ? rho / a.group : 0;
+      h = s.kvh * a.group + (rho < total ? rho - r * a.group : 0);
+    };
+    // The tile's query rows to shared memory, in the swizzled layout of the
+    // products: the warp copies its 32 rows (PAIR: all channels, else its
+    // half), kRow lanes a row; rows past the last are zero.
+    auto q_fetch = [&]() {
+      constexpr int kCols = PAIR ? D : D / 2, kRow = kCols / 8;
+      const int64_t off = rho < total ? (r * a.q_row + h * a.q_head) * 2 : -1;
+      unsigned char* q = smem + (PAIR ? st * (kTcRows * D * 2) : 0);
+      const int c = (PAIR ? 0 : st * kCols) + 8 * (lane % kRow);
+#pragma unroll 4
+      for (int i = 0; i < 32; i += 32 / kRow) {
+        const int row = i + lane / kRow, tr = (warp & 3) * 32 + row;
+        const int64_t at = __shfl_sync(0xffffffffu, off, row);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(
+                         q + (c >> 6) * (kTcRows * 128) + tr * 128 + ((((c & 63) >> 3) ^ (tr & 7)) << 4))),
+                     "l"(static_cast<const char*>(a.q) + (at < 0 ? 0 : at + 2 * c)), "r"(at < 0 ? 0 : 16)
+                     : "memory");
+      }
+    };
+    auto q_ready = [&]() {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async();
+      mbar_arrive(q_full);
+    };
+    int u_next;
+    Segment s = segment_at(a, u_begin, u_begin, u_end, &u_next);
+    place(s);
+    if (s.nb > 0) q_fetch();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot, lanes = static_cast<uint32_t>(warp & 3) << 21;   // TMEM lane 32 (warp % 4)
+    const uint32_t ts = tmem + 128 * st + lanes, to = tmem + 256 + 128 * st + lanes;
     uint32_t ph = 0, oph = 0;
     float2* ml = reinterpret_cast<float2*>(smem + Ly::kMl);
-    for (int64_t u = u_begin; u < u_end;) {
-      const Segment s = segment_at(a, u, u_begin, u_end, &u);
-      const int tile_row = PAIR ? st * kTcRows + t : t;
-      const int rho = s.rho0 + tile_row;
-      const bool live = rho < total;
-      const bool warp_live = rho - lane < total;
-      const int r = live ? rho / a.group : 0, h = s.kvh * a.group + (live ? rho - r * a.group : 0);
+    if (s.nb > 0) q_ready();
+    for (;;) {
+      const bool live = rho < total, warp_live = rho - lane < total;
       const int vis = live ? visible(a, r) : 0;
       const int n_own = s.nb == 0 ? 0 : PAIR ? s.nb : (s.nb + 1 - st) >> 1;   // blocks of this stream
-      if (s.nb > 0) {
-        // the tile's query rows, in the swizzled layout of the products
-        constexpr int kCols = PAIR ? D : D / 2;
-        const int c0 = PAIR ? 0 : st * kCols;
-        unsigned char* q = smem + (PAIR ? st * (kTcRows * D * 2) : 0);
-        const char* src = static_cast<const char*>(a.q) + (r * a.q_row + h * a.q_head + c0) * 2;
-#pragma unroll
-        for (int i = 0; i < kCols / 8; ++i) {
-          const int c = c0 + 8 * i;
-          const uint4 v = live ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(q + (c >> 6) * (kTcRows * 128) + t * 128 + ((((c & 63) >> 3) ^ (t & 7)) << 4)) = v;
-        }
-        fence_proxy_async();
-        mbar_arrive(q_full);
-      }
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n_own; ++j) {
         ok = ok && __all_sync(0xffffffffu, wait_or(s_full + st, ph, dead));
         ph ^= 1;
         tc_fence_after();
-        if (ok && warp_live) {
-          const int t0 = (s.b0 + (PAIR ? j : 2 * j + st)) * kTcBlock;
-          uint32_t x[128];
-          tmem_ld128(ts, x);
-          if (__any_sync(0xffffffffu, t0 + kTcBlock > vis)) {
+        const bool work = ok && warp_live;
+        uint32_t x[64];
+        float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+        float mb = 0.f;
+        bool edge = false;
+        const int t0 = (s.b0 + (PAIR ? j : 2 * j + st)) * kTcBlock;
+        auto fetch = [&](int c) {
+          tmem_ld64(ts + c, x);
+          if (edge) {
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (t0 + i >= vis) x[i] = 0xff800000u;
+            for (int i = 0; i < 64; ++i)
+              if (t0 + c + i >= vis) x[i] = 0xff800000u;
           }
+        };
+        if (work) {
+          // 64 columns at a time (128 scores would not fit the registers): the
+          // upper half for its maximum only, then the lower half, kept.  The
+          // loops over halves stay loops: the code is fetched anew by every
+          // launch, and its size shows in the first block's time.
+          edge = __any_sync(0xffffffffu, t0 + kTcBlock > vis);
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int c = 64; c >= 0; c -= 64) {
+            fetch(c);
 #pragma unroll
-          for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(x[i]));
+            for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(x[i]));
+          }
           const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2 - bias;
           const bool raise = mt > m + kRaise;
           if (__any_sync(0xffffffffu, raise)) {
@@ -497,27 +580,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
               }
             }
           }
-          const float mb = m == -INFINITY ? 0.f : -m;
-          float sum[4] = {};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float p0 = ex2(fmaf(__uint_as_float(x[32 * c + 2 * i]), a.scale2, mb));
-              const float p1 = ex2(fmaf(__uint_as_float(x[32 * c + 2 * i + 1]), a.scale2, mb));
-              sum[i & 1] += p0;
-              sum[2 + (i & 1)] += p1;
-              w[i] = pack16<BF>(p0, p1);
-            }
-            tmem_st16(ts + 16 * c, w);
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_wait_st();
+          mb = m == -INFINITY ? 0.f : -m;
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + st);
+#pragma unroll 1
+        for (int c = 0; c < kTcBlock; c += 64) {
+          if (work) {
+            if (c > 0) fetch(c);
+            // weights of tokens c .. c + 63 to columns c / 2 .. of P, which
+            // lie over scores that are in registers or done by then
+            const float2 sc = make_float2(a.scale2, a.scale2), mb2 = make_float2(mb, mb);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              uint32_t w[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 y = fma2(
+                    make_float2(__uint_as_float(x[32 * g + 2 * i]), __uint_as_float(x[32 * g + 2 * i + 1])), sc, mb2);
+                const float2 p = make_float2(ex2(y.x), ex2(y.y));
+                sum[i & 1] = add2(sum[i & 1], p);
+                w[i] = pack16<BF>(p.x, p.y);
+              }
+              tmem_st16(ts + c / 2 + 16 * g, w);
+            }
+            tmem_wait_st();
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive((c == 0 ? p_half : p_full) + st);
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      }
+      const Segment done_s = s;
+      const int done_rho = rho;
+      const bool more = u_next < u_end;
+      if (more) {
+        s = segment_at(a, u_next, u_begin, u_end, &u_next);
+        place(s);
       }
       if (n_own > 0) {
         ok = ok && __all_sync(0xffffffffu, wait_or(o_full + st, oph, dead));
@@ -529,6 +627,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
         l = __int_as_float(0x7fc00000);
       }
       if constexpr (PAIR) {
+        if (more && s.nb > 0) {   // this stream's products with the old rows are done
+          q_fetch();
+          q_ready();
+        }
         if (warp_live) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -537,7 +639,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
             if (ok && n_own > 0) tmem_ld32(to + c, x);
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = ok && n_own > 0 ? __uint_as_float(x[i]) : 0.f;
-            if (live) store_row<D, 32, BF>(a, s, rho, tile_row, m, l, c, o, c == 0);
+            if (live) store_row<D, 32, BF>(a, done_s, done_rho, tile_row, m, l, c, o, c == 0);
           }
         }
         tc_fence_before();
@@ -545,14 +647,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
         // join the streams: this thread takes half of the row's channels
         ml[st * kTcRows + t] = make_float2(m, l);
         named_sync(1, 256);
+        if (more && s.nb > 0) {   // both streams' products are done
+          q_fetch();
+          q_ready();
+        }
         if (warp_live) {
           const float2 y = ml[(st ^ 1) * kTcRows + t];
-          float top = fmaxf(m, y.x);
+          const float top = fmaxf(m, y.x);
           const float base = top == -INFINITY ? 0.f : top;
           const float fo = ex2(m - base), fy = ex2(y.x - base);
           const float f0 = st == 0 ? fo : fy, f1 = st == 0 ? fy : fo;
           const float ls = fo * l + fy * y.y;
-          const bool h0 = ok && s.nb > 0, h1 = ok && s.nb > 1;
+          const bool h0 = ok && done_s.nb > 0, h1 = ok && done_s.nb > 1;
 #pragma unroll 1
           for (int c = st * (D / 2); c < (st + 1) * (D / 2); c += 32) {
             uint32_t x[32];
@@ -565,50 +671,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
 #pragma unroll
               for (int i = 0; i < 32; ++i) o[i] = fmaf(f1, __uint_as_float(x[i]), o[i]);
             }
-            if (live) store_row<D, 32, BF>(a, s, rho, tile_row, top, ls, c, o, c == 0);
+            if (live) store_row<D, 32, BF>(a, done_s, done_rho, tile_row, top, ls, c, o, c == 0);
           }
         }
         tc_fence_before();
-        named_sync(1, 256);
+        if (more) named_sync(1, 256);   // the sums may be overwritten
       }
+      if (!more) break;
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(*tmem_slot, 512);
   }
 }
 
 // ── join ────────────────────────────────────────────────────────────────
-// One warp per (row, head): the partials and the row's own state.  TC: the
-// partials of the tensor-core form, rows of whole tiles are done already;
-// else those of the FMA form, [split][row].
-template <bool TC>
-__global__ void __launch_bounds__(256) prefix_combine_kernel(const PrefixArgs a, const int splits) {
+// One warp per (row, head): the partials and the row's own state.  Rows of
+// tiles that one CTA held whole are done already.  Lane s finds partial s
+// (of up to 32 at a time) and its weight; then the partials are read eight at
+// a time, a row of D floats per warp load.
+template <int D>
+__global__ void __launch_bounds__(256) prefix_combine_kernel(const PrefixArgs a) {
+  constexpr int V = D / 32;
+  struct alignas(4 * V) Vec {
+    float v[V];
+  };
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t n = static_cast<int64_t>(a.rows) * a.heads;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, D = a.p.head_dim, dt = a.p.dtype;
+  const int lane = threadIdx.x & 31;
   if (i >= n) return;
-  int parts = splits, c0 = 0, tile_row = 0;
-  int64_t u0 = 0;
-  if constexpr (TC) {
-    const int r = static_cast<int>(i / a.heads), h = static_cast<int>(i - static_cast<int64_t>(r) * a.heads);
-    const int kvh = h / a.group, rho = r * a.group + h % a.group;
-    tile_row = rho % a.sp.tile_rows;
-    u0 = (static_cast<int64_t>(kvh) * a.sp.tiles + rho / a.sp.tile_rows) * a.sp.blocks;
-    c0 = a.sp.cta_of(u0);
-    parts = a.sp.cta_of(u0 + a.sp.blocks - 1) - c0 + 1;
-    if (parts == 1) return;
-  }
+  const int r = static_cast<int>(i / a.heads), h = static_cast<int>(i - static_cast<int64_t>(r) * a.heads);
+  const int kvh = h / a.group, rho = r * a.group + h % a.group;
+  const int tile_row = rho % a.sp.tile_rows;
+  const int u0 = (kvh * a.sp.tiles + rho / a.sp.tile_rows) * a.sp.blocks;
+  const int c0 = a.sp.cta_of(u0), parts = a.sp.cta_of(u0 + a.sp.blocks - 1) - c0 + 1;
+  if (parts == 1) return;
   auto at = [&](int s) -> int64_t {
-    if constexpr (TC) {
-      const int64_t slot = 2 * (c0 + s) + (a.sp.start(c0 + s) >= u0 ? 0 : 1);
-      return slot * a.sp.tile_rows + tile_row;
-    } else {
-      return s * n + i;
-    }
+    const int64_t slot = 2 * (c0 + s) + (a.sp.start(c0 + s) >= u0 ? 0 : 1);
+    return slot * a.sp.tile_rows + tile_row;
   };
   const float lt = a.tail ? a.tail_lse[i] * kL2e : -INFINITY;
   float m = -INFINITY;
@@ -618,12 +722,63 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const PrefixArgs a,
   // a state of no tokens (lse -inf) takes no part, whatever its values hold
   const bool own = lt != -INFINITY;
   const float wt = own ? exp2f(lt - m) : 0.f;
+  float L = 0.f, o[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) o[k] = own ? wt * load_act(a.tail, i * D + V * lane + k, a.p.dtype) : 0.f;
+  for (int s0 = 0; s0 < parts; s0 += 32) {
+    int64_t p = 0;
+    float w = 0.f;
+    if (s0 + lane < parts) {
+      p = at(s0 + lane);
+      const float2 x = a.ml[p];
+      w = exp2f(x.x - m);
+      L = fmaf(w, x.y, L);
+    }
+    const int cnt = min(32, parts - s0);
+    for (int s = 0; s < cnt; s += 8) {
+      Vec v[8];
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        f[j] = __shfl_sync(0xffffffffu, w, (s + j) & 31);
+        const int64_t q = __shfl_sync(0xffffffffu, p, (s + j) & 31);
+        if (s + j < cnt && f[j] != 0.f) v[j] = reinterpret_cast<const Vec*>(a.po + q * D)[lane];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (s + j < cnt && f[j] != 0.f) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) o[k] = fmaf(f[j], v[j].v[k], o[k]);
+        }
+    }
+  }
+  L = warp_sum(L) + wt;
+  const bool any = L > 0.f || L != L;
+  const float inv = any ? 1.f / L : 0.f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) store_act(a.out, i * D + V * lane + k, o[k] * inv, a.p.dtype);
+  if (a.lse && lane == 0) a.lse[i] = any ? (m + log2f(L)) * kLn2 : -INFINITY;
+}
+
+// The same for the FMA form's partials, [split][row].
+__global__ void __launch_bounds__(256) prefix_fma_combine_kernel(const PrefixArgs a, const int splits) {
+  const int64_t n = static_cast<int64_t>(a.rows) * a.heads;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, D = a.p.head_dim, dt = a.p.dtype;
+  if (i >= n) return;
+  const float lt = a.tail ? a.tail_lse[i] * kL2e : -INFINITY;
+  float m = -INFINITY;
+  for (int s = lane; s < splits; s += 32) m = fmaxf(m, a.ml[s * n + i].x);
+  m = fmaxf(warp_max(m), lt);
+  if (m == -INFINITY) m = 0.f;
+  const bool own = lt != -INFINITY;
+  const float wt = own ? exp2f(lt - m) : 0.f;
   float L = wt, o[kFmaMaxD / 32];
 #pragma unroll
   for (int k = 0; k < kFmaMaxD / 32; ++k)
     o[k] = own && lane + 32 * k < D ? wt * load_act(a.tail, i * D + lane + 32 * k, dt) : 0.f;
-  for (int s = 0; s < parts; ++s) {
-    const int64_t p = at(s);
+  for (int s = 0; s < splits; ++s) {
+    const int64_t p = s * n + i;
     const float2 x = a.ml[p];
     const float w = exp2f(x.x - m);
     L = fmaf(w, x.y, L);
@@ -642,16 +797,6 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const PrefixArgs a,
 }
 
 // ── host ────────────────────────────────────────────────────────────────
-int sm_count() {
-  static thread_local int count[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (count[dev] == 0 &&
-      cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return count[dev];
-}
-
 // FMA form: splits of the prefix, enough CTAs for the GPU, at least 128 tokens each
 int fma_splits(const carekv_prefix_t& p, int rows, int heads) {
   const int64_t ctas = static_cast<int64_t>(p.num_kv_heads) *
@@ -660,15 +805,34 @@ int fma_splits(const carekv_prefix_t& p, int rows, int heads) {
   return std::max(1, std::min(want, (p.tokens + 127) / 128));
 }
 
-Split tc_split(const carekv_prefix_t& p, int rows, int heads) {
-  Split s;
+// Every CTA works on one SM for the whole launch.  Either the CTAs of a tile
+// share it evenly, or all CTAs share all units evenly and most of them cross
+// a tile's end, which costs about kCross units (the state of one tile written
+// out, the pipeline filled for the next).
+constexpr int kCross = 4;
+
+bool tc_split(const carekv_prefix_t& p, int rows, int heads, Split* s) {
   const int64_t per_head = static_cast<int64_t>(rows) * (heads / p.num_kv_heads);
-  s.tile_rows = per_head <= kTcRows ? kTcRows : 2 * kTcRows;
-  s.tiles = static_cast<int>((per_head + s.tile_rows - 1) / s.tile_rows);
-  s.blocks = (p.tokens + kTcBlock - 1) / kTcBlock;
-  s.units = static_cast<int64_t>(s.tiles) * p.num_kv_heads * s.blocks;
-  s.ctas = static_cast<int>(std::min<int64_t>(sm_count(), s.units));
-  return s;
+  s->tile_rows = per_head <= kTcRows ? kTcRows : 2 * kTcRows;
+  s->tiles = static_cast<int>((per_head + s->tile_rows - 1) / s->tile_rows);
+  s->blocks = (p.tokens + kTcBlock - 1) / kTcBlock;
+  const int64_t tiles = static_cast<int64_t>(s->tiles) * p.num_kv_heads, units = tiles * s->blocks;
+  if (units > (1 << 30)) return false;
+  s->units = static_cast<int>(units);
+  const int sms = sm_count();
+  const int per = static_cast<int>(std::min<int64_t>(tiles <= sms ? sms / tiles : 0, s->blocks));
+  const int64_t even = (units + sms - 1) / sms;
+  if (per > 0 && (s->blocks + per - 1) / per <= even + kCross) {
+    s->group = s->blocks;
+    s->per = per;
+    s->ctas = static_cast<int>(tiles) * per;
+  } else {
+    s->group = s->units;
+    s->per = s->ctas = static_cast<int>(std::min<int64_t>(sms, units));
+  }
+  s->base = s->group / s->per;
+  s->rem = s->group % s->per;
+  return true;
 }
 
 bool tc_shape(const carekv_prefix_t& p) {
@@ -711,8 +875,7 @@ cudaError_t launch_tc(const PrefixArgs& a, const CUtensorMap& km, const CUtensor
                       cudaStream_t st) {
   constexpr int smem = TcLayout<D, PAIR>::kBytes;
   static_assert(smem <= 232448, "shared memory of one CTA");
-  const cudaError_t e =
-      cudaFuncSetAttribute(prefix_tc_kernel<D, BF, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = allow_smem<smem>(prefix_tc_kernel<D, BF, PAIR>);
   if (e != cudaSuccess) return e;
   prefix_tc_kernel<D, BF, PAIR><<<a.sp.ctas, kTcThreads, smem, st>>>(a, km, vm, kh, vh);
   return cudaGetLastError();
@@ -724,11 +887,20 @@ cudaError_t launch_tc(const PrefixArgs& a, const CUtensorMap& km, const CUtensor
                                    : launch_tc<D, BF, true>(a, km, vm, kh, vh, st);
 }
 
-template <bool TC>
-cudaError_t launch_combine(const PrefixArgs& a, int splits, cudaStream_t st) {
+// The join starts while the products' last CTAs run and waits for them itself.
+cudaError_t launch_combine(const PrefixArgs& a, cudaStream_t st) {
   const int64_t n = static_cast<int64_t>(a.rows) * a.heads;
-  prefix_combine_kernel<TC><<<static_cast<unsigned>((n + 7) / 8), 256, 0, st>>>(a, splits);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((n + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return a.p.head_dim == 128 ? cudaLaunchKernelEx(&cfg, prefix_combine_kernel<128>, a)
+                             : cudaLaunchKernelEx(&cfg, prefix_combine_kernel<64>, a);
 }
 
 }  // namespace
@@ -737,10 +909,9 @@ cudaError_t launch_combine(const PrefixArgs& a, int splits, cudaStream_t st) {
 size_t prefix_workspace_bytes(const carekv_prefix_t& p, int rows, int heads) {
   const size_t row = static_cast<size_t>(p.head_dim + 2) * sizeof(float);
   size_t n = static_cast<size_t>(fma_splits(p, rows, heads)) * rows * heads;
-  if (tc_shape(p) && rows > 0) {
-    const Split s = tc_split(p, rows, heads);
+  Split s;
+  if (tc_shape(p) && rows > 0 && tc_split(p, rows, heads, &s))
     n = std::max(n, static_cast<size_t>(2) * s.ctas * s.tile_rows);
-  }
   return n * row;
 }
 
@@ -768,9 +939,8 @@ cudaError_t launch_prefix(const carekv_prefix_t& p, const void* q, int64_t q_row
                       static_cast<uintptr_t>(q_head * 2);
   CUtensorMap km, vm;
   int kh, vh;
-  if (tc_shape(p) && (m & 15) == 0 && tensor_map(&km, p.k, p, p.k_stride, &kh) &&
+  if (tc_shape(p) && (m & 15) == 0 && tc_split(p, rows, heads, &a.sp) && tensor_map(&km, p.k, p, p.k_stride, &kh) &&
       tensor_map(&vm, p.v, p, p.v_stride, &vh)) {
-    a.sp = tc_split(p, rows, heads);
     a.po = static_cast<float*>(ws);
     a.ml = reinterpret_cast<float2*>(a.po + static_cast<size_t>(2) * a.sp.ctas * a.sp.tile_rows * p.head_dim);
     const bool bf = p.dtype == CAREKV_BF16;
@@ -782,7 +952,7 @@ cudaError_t launch_prefix(const carekv_prefix_t& p, const void* q, int64_t q_row
     // no tile is cut when every CTA starts on a tile
     bool cut = false;
     for (int c = 1; c < a.sp.ctas && !cut; ++c) cut = a.sp.start(c) % a.sp.blocks != 0;
-    return cut ? launch_combine<true>(a, 0, st) : cudaSuccess;
+    return cut ? launch_combine(a, st) : cudaSuccess;
   }
   const int splits = p.tokens > 0 ? fma_splits(p, rows, heads) : 0;
   a.po = static_cast<float*>(ws);
@@ -790,14 +960,15 @@ cudaError_t launch_prefix(const carekv_prefix_t& p, const void* q, int64_t q_row
   if (splits) {
     const int split_tokens = ((p.tokens + splits - 1) / splits + kFmaTok - 1) / kFmaTok * kFmaTok;
     const size_t smem = (kFmaRows * p.head_dim + kFmaTok * (2 * p.head_dim + 1)) * sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(prefix_fma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
+    cudaError_t e = allow_smem<96 * 1024>(prefix_fma_kernel);
     if (e != cudaSuccess) return e;
     const dim3 grid((rows * a.group + kFmaRows - 1) / kFmaRows, p.num_kv_heads, splits);
     prefix_fma_kernel<<<grid, kFmaRows * 32, smem, st>>>(a, split_tokens);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  return launch_combine<false>(a, splits, st);
+  prefix_fma_combine_kernel<<<static_cast<unsigned>((n + 7) / 8), 256, 0, st>>>(a, splits);
+  return cudaGetLastError();
 }
 
 }  // namespace carekv

@@ -37,18 +37,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld128(uint32_t addr, uint32_t (&r)[128]) {
+__device__ __forceinline__ void tmem_ld64(uint32_t addr, uint32_t (&r)[64]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
       "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,"
-      "%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,"
-      "%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,%96,%97,%98,%99,%100,"
-      "%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,"
-      "%122,%123,%124,%125,%126,%127}, [%128];\n"
+      "%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
       "tcgen05.wait::ld.sync.aligned;"
       : CAREKV_R8(r, 0), CAREKV_R8(r, 8), CAREKV_R8(r, 16), CAREKV_R8(r, 24), CAREKV_R8(r, 32), CAREKV_R8(r, 40),
-        CAREKV_R8(r, 48), CAREKV_R8(r, 56), CAREKV_R8(r, 64), CAREKV_R8(r, 72), CAREKV_R8(r, 80), CAREKV_R8(r, 88),
-        CAREKV_R8(r, 96), CAREKV_R8(r, 104), CAREKV_R8(r, 112), CAREKV_R8(r, 120)
+        CAREKV_R8(r, 48), CAREKV_R8(r, 56)
       : "r"(addr)
       : "memory");
 }
@@ -82,26 +78,40 @@ __host__ __device__ constexpr uint32_t mma_idesc(int m, int n, bool bf16, bool m
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (mn_b ? 1u << 16 : 0u) |
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
-// One thread.  D (TMEM) = A (shared) . B (shared) [+ D]
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+// One lane of a converged warp, the same one every time (its products and
+// commits are then ordered).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+  return is;
+}
+// The products are predicated on `lead` instead of standing in a branch of
+// one lane: all operands but the predicate are the same in the whole warp,
+// so they can stay in uniform registers, where the instruction wants them
+// (a single lane's branch took 0.6 us to issue eight products).
+// D (TMEM) = A (shared) . B (shared) [+ D]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc, uint32_t lead) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)), "r"(lead)
       : "memory");
 }
 // D (TMEM) = A (TMEM, pairs of 16-bit values per column) . B (shared) [+ D]
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc, uint32_t lead) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)), "r"(lead)
       : "memory");
 }
-// One arrival on `bar` when every product this thread issued has completed.
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-               : "memory");
+// One arrival on `bar` when every product the lead lane issued has completed.
+__device__ __forceinline__ void mma_commit(uint64_t* bar, uint32_t lead) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_addr(bar)),
+      "r"(lead)
+      : "memory");
 }
 
 // ── tiled loads ─────────────────────────────────────────────────────────

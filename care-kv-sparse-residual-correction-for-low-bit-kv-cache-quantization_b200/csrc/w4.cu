@@ -13,6 +13,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "launch.h"
 #include "ptx.cuh"
 
 namespace cg = cooperative_groups;
@@ -541,7 +542,7 @@ cudaError_t launch_wide(const carekv_w4_t& w, const void* x, int64_t ldx, int M,
   constexpr int kPerSm = MT == 2 ? 2 : 1;
   const int splits = std::max(1, std::min({8, kPerSm * 148 / (blocks * cols), kt_n / 4}));
   auto kernel = w4_wide_kernel<DT, NS, MT, RT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ly::kBytes);
+  const cudaError_t e = allow_smem<Ly::kBytes>(kernel);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks * splits, cols);
