@@ -21,23 +21,25 @@ namespace {
 constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // How the prefix is cut: a unit is one block of tokens for one tile of rows,
-// units are numbered tile by tile (tiles of kv head 0 first).  Every group of
-// `group` consecutive units is shared evenly by `per` CTAs; a group is one
-// tile, or all units.  What a CTA has of a tile it does not hold whole is a
-// partial, in slot 2c if the tile is the CTA's first, else in slot 2c + 1.
+// units are numbered tile by tile (tiles of kv head 0 first).  CTA c takes
+// `whole` whole tiles, from tile c * whole on, and a share of the units of the
+// tiles after those: every group of `group` consecutive units is shared
+// evenly by `per` CTAs, a group being one tile or all that is left.  What a
+// CTA has of a tile it does not hold whole is a partial, in slot 2c if it
+// begins the CTA's share, else in slot 2c + 1.
 struct Split {
   int tile_rows;    // rows of a kv head per tile
   int tiles;        // tiles per kv head
   int blocks;       // units per tile
-  int units;
   int ctas;
+  int whole, first;            // first: first shared unit, ctas * whole * blocks
   int group, per, base, rem;   // base, rem = group / per, group % per
-  __host__ __device__ int start(int c) const {
+  __host__ __device__ int start(int c) const {   // first unit of CTA c's share
     const int g = c / per, i = c - g * per;
-    return g * group + i * base + (i < rem ? i : rem);
+    return first + g * group + i * base + (i < rem ? i : rem);
   }
-  __host__ __device__ int cta_of(int u) const {
-    const int g = u / group, v = u - g * group, cut = rem * (base + 1);
+  __host__ __device__ int cta_of(int u) const {   // of a shared unit
+    const int g = (u - first) / group, v = u - first - g * group, cut = rem * (base + 1);
     return g * per + (v < cut ? v / (base + 1) : rem + (v - cut) / base);
   }
 };
@@ -146,6 +148,9 @@ __global__ void __launch_bounds__(kFmaRows * 32) prefix_fma_kernel(const PrefixA
 // ulp per weight, independent between tokens, like the result's own rounding.
 constexpr int kTcThreads = 320, kTcRows = 128, kTcBlock = 128;
 constexpr float kRaise = 8.f;
+// Of 8 pairs of weights, those computed on the FMA pipe: the 16 special-function
+// lanes of an SM would take 2048 cycles for a block's 256 rows x 128 weights.
+constexpr int kFmaOf8 = 3;
 
 template <int D, bool PAIR>
 struct TcLayout {
@@ -179,17 +184,30 @@ struct Segment {
   int slot;           // partial slot, -1: the CTA holds the whole tile
 };
 
-// The part of a tile in [u, u_end); the whole warp calls it.
-__device__ __forceinline__ Segment segment_at(const PrefixArgs& a, int u, int u_begin, int u_end, int* next) {
+// A CTA's units: its whole tiles, then its share.
+struct Units {
+  int whole_end, share, end;
+  __device__ __forceinline__ int begin(const Split& sp) {
+    const int c = blockIdx.x;
+    whole_end = (c + 1) * sp.whole * sp.blocks;
+    share = sp.start(c);
+    end = sp.start(c + 1);
+    return sp.whole ? c * sp.whole * sp.blocks : share;
+  }
+};
+
+// The part of a tile from unit u on (u < un.end); the whole warp calls it.
+__device__ __forceinline__ Segment segment_at(const PrefixArgs& a, const Units& un, int u, int* next) {
   Segment s;
   const int tile = u / a.sp.blocks, tile0 = tile * a.sp.blocks;
-  const int end = min(u_end, tile0 + a.sp.blocks);
-  *next = end;
+  const bool whole = u < un.share;
+  const int end = whole ? tile0 + a.sp.blocks : min(un.end, tile0 + a.sp.blocks);
+  *next = whole && end == un.whole_end ? un.share : end;
   s.kvh = tile / a.sp.tiles;
   s.rho0 = (tile - s.kvh * a.sp.tiles) * a.sp.tile_rows;
   s.b0 = u - tile0;
   s.nb = end - u;
-  s.slot = end - u == a.sp.blocks ? -1 : 2 * static_cast<int>(blockIdx.x) + (u == u_begin ? 0 : 1);
+  s.slot = end - u == a.sp.blocks ? -1 : 2 * static_cast<int>(blockIdx.x) + (u == un.share ? 0 : 1);
   s.top = a.p.tokens;
   if (a.lengths) {
     const int last = min(s.rho0 + a.sp.tile_rows, a.rows * a.group) - 1;
@@ -219,6 +237,27 @@ __device__ __forceinline__ float2 add2(float2 x, float2 y) {
   asm("add.rn.f32x2 %0, %1, %2;"
       : "=l"(*reinterpret_cast<uint64_t*>(&r))
       : "l"(*reinterpret_cast<uint64_t*>(&x)), "l"(*reinterpret_cast<uint64_t*>(&y)));
+  return r;
+}
+// 2^y of two values on the FMA pipe, y >= -126 or clamped to it: y = n + f
+// with n the nearest integer (by adding 1.5 2^23), |f| <= 1/2, a degree-4
+// polynomial for 2^f (fitted for the least relative error, 2.6e-6) and n added
+// to its exponent (Cody and Waite's scheme).
+__device__ __forceinline__ float2 ex2_fma(float2 y) {
+  y = make_float2(fmaxf(y.x, -126.f), fmaxf(y.y, -126.f));
+  const float2 big = make_float2(12582912.f, 12582912.f), nbig = make_float2(-12582912.f, -12582912.f);
+  const float2 r = add2(y, big), n = add2(r, nbig);
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), y);
+  float2 p = fma2(f, make_float2(0x1.3997d4p-7f, 0x1.3997d4p-7f), make_float2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+  p = fma2(p, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  p = fma2(p, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  p = fma2(p, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
+}
+__device__ __forceinline__ float max_nan(float x, float y) {   // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
   return r;
 }
 template <bool BF>
@@ -301,7 +340,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Ly::kBars);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int u_begin = a.sp.start(blockIdx.x), u_end = a.sp.start(blockIdx.x + 1);
+  Units un;
+  const int u_begin = un.begin(a.sp);
   bool ok = true;
 
   if (warp == 8) {
@@ -324,6 +364,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
       fence_mbar_init();
     }
     __syncwarp();
+    // With one tile per kv head every K / V byte is read once: it leaves the
+    // L2 first (16 rows on 32768 tokens 29.3 -> 27.0 us).  With several, the
+    // other tiles' CTAs find it there (2048 rows on 8192: 258 against 264 us).
+    const uint64_t policy = l2_evict_first();
     int cnt = 0;
     bool synced = false;
     auto sync_once = [&]() {
@@ -345,12 +389,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
         mbar_expect_tx(full + slot, Ly::kSlot);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_3d(dst + c * (kTcBlock * 128), map, 64 * c, block * kTcBlock, z, full + slot);
+          if constexpr (PAIR) tma_load_3d(dst + c * (kTcBlock * 128), map, 64 * c, block * kTcBlock, z, full + slot);
+          else tma_load_3d_pol(dst + c * (kTcBlock * 128), map, 64 * c, block * kTcBlock, z, full + slot, policy);
       }
       ++cnt;
     };
-    for (int u = u_begin; u < u_end && ok;) {
-      const Segment s = segment_at(a, u, u_begin, u_end, &u);
+    for (int u = u_begin; u < un.end && ok;) {
+      const Segment s = segment_at(a, un, u, &u);
       const int zk = s.kvh * k_heads, zv = s.kvh * v_heads;
       if (s.nb > 0) load(&kmap, zk, s.b0);
       if (!PAIR && s.nb > 1) load(&kmap, zk, s.b0 + 1);
@@ -415,8 +460,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
     auto finish = [&](int stream) {
       if (ok) mma_commit(o_full + stream, lead);
     };
-    for (int u = u_begin; u < u_end && ok;) {
-      const Segment s = segment_at(a, u, u_begin, u_end, &u);
+    for (int u = u_begin; u < un.end && ok;) {
+      const Segment s = segment_at(a, un, u, &u);
       if (s.nb == 0) continue;
       wait(q_full, seg & 1);
       ++seg;
@@ -515,7 +560,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
       mbar_arrive(q_full);
     };
     int u_next;
-    Segment s = segment_at(a, u_begin, u_begin, u_end, &u_next);
+    Segment s = segment_at(a, un, u_begin, &u_next);
     place(s);
     if (s.nb > 0) q_fetch();
     tc_fence_before();
@@ -560,10 +605,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
           for (int c = 64; c >= 0; c -= 64) {
             fetch(c);
 #pragma unroll
-            for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(x[i]));
+            for (int i = 0; i < 64; ++i) mx[i & 3] = max_nan(mx[i & 3], __uint_as_float(x[i]));
           }
-          const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2 - bias;
-          const bool raise = mt > m + kRaise;
+          float mt = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * a.scale2 - bias;
+          if (mt == INFINITY) mt = __int_as_float(0x7fc00000);   // the row's weights are inf - inf
+          const bool raise = !(mt <= m + kRaise);                // NaN raises too and makes all weights NaN
           if (__any_sync(0xffffffffu, raise)) {
             const float mn = raise ? mt : m;
             const float f = raise ? ex2(m - mn) : 1.f;
@@ -596,7 +642,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
               for (int i = 0; i < 16; ++i) {
                 const float2 y = fma2(
                     make_float2(__uint_as_float(x[32 * g + 2 * i]), __uint_as_float(x[32 * g + 2 * i + 1])), sc, mb2);
-                const float2 p = make_float2(ex2(y.x), ex2(y.y));
+                const float2 p = i % 8 < kFmaOf8 ? ex2_fma(y) : make_float2(ex2(y.x), ex2(y.y));
                 sum[i & 1] = add2(sum[i & 1], p);
                 w[i] = pack16<BF>(p.x, p.y);
               }
@@ -608,13 +654,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
           __syncwarp();
           if (lane == 0) mbar_arrive((c == 0 ? p_half : p_full) + st);
         }
-        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        // a row that has seen nothing has no weight (ex2_fma's least is 2^-126)
+        if (m != -INFINITY) l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
       const Segment done_s = s;
       const int done_rho = rho;
-      const bool more = u_next < u_end;
+      const bool more = u_next < un.end;
       if (more) {
-        s = segment_at(a, u_next, u_begin, u_end, &u_next);
+        s = segment_at(a, un, u_next, &u_next);
         place(s);
       }
       if (n_own > 0) {
@@ -689,51 +736,70 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
 }
 
 // ── join ────────────────────────────────────────────────────────────────
-// One warp per (row, head): the partials and the row's own state.  Rows of
-// tiles that one CTA held whole are done already.  Lane s finds partial s
-// (of up to 32 at a time) and its weight; then the partials are read eight at
-// a time, a row of D floats per warp load.
-template <int D>
+// A CTA per 8 rows of a shared tile, a warp per (row, head): the partials and
+// the row's own state.  Lane s finds partial s (of up to 32 at a time) and its
+// weight; then the partials are read eight at a time, a row of D floats per
+// warp load.
+template <int D, bool BF>
 __global__ void __launch_bounds__(256) prefix_combine_kernel(const PrefixArgs a) {
   constexpr int V = D / 32;
   struct alignas(4 * V) Vec {
     float v[V];
   };
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t n = static_cast<int64_t>(a.rows) * a.heads;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (i >= n) return;
-  const int r = static_cast<int>(i / a.heads), h = static_cast<int>(i - static_cast<int64_t>(r) * a.heads);
-  const int kvh = h / a.group, rho = r * a.group + h % a.group;
-  const int tile_row = rho % a.sp.tile_rows;
-  const int u0 = (kvh * a.sp.tiles + rho / a.sp.tile_rows) * a.sp.blocks;
-  const int c0 = a.sp.cta_of(u0), parts = a.sp.cta_of(u0 + a.sp.blocks - 1) - c0 + 1;
-  if (parts == 1) return;
-  auto at = [&](int s) -> int64_t {
-    const int64_t slot = 2 * (c0 + s) + (a.sp.start(c0 + s) >= u0 ? 0 : 1);
-    return slot * a.sp.tile_rows + tile_row;
+  struct alignas(2 * V) Vec16 {
+    uint32_t v[V / 2];
   };
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int ctas = a.sp.tile_rows / 8;
+  const int tile = a.sp.ctas * a.sp.whole + static_cast<int>(blockIdx.x) / ctas;
+  const int u0 = tile * a.sp.blocks;
+  const int c0 = a.sp.cta_of(u0), parts = a.sp.cta_of(u0 + a.sp.blocks - 1) - c0 + 1;
+  const int kvh = tile / a.sp.tiles;
+  const int tile_row = (static_cast<int>(blockIdx.x) % ctas) * 8 + (threadIdx.x >> 5);
+  const int rho = (tile - kvh * a.sp.tiles) * a.sp.tile_rows + tile_row;
+  if (parts == 1 || rho >= a.rows * a.group) return;
+  const int r = rho / a.group;
+  const int64_t i = static_cast<int64_t>(r) * a.heads + kvh * a.group + (rho - r * a.group);
+  auto at = [&](int s) { return (2 * (c0 + s) + (a.sp.start(c0 + s) >= u0 ? 0 : 1)) * a.sp.tile_rows + tile_row; };
   const float lt = a.tail ? a.tail_lse[i] * kL2e : -INFINITY;
-  float m = -INFINITY;
-  for (int s = lane; s < parts; s += 32) m = fmaxf(m, a.ml[at(s)].x);
-  m = fmaxf(warp_max(m), lt);
-  if (m == -INFINITY) m = 0.f;
   // a state of no tokens (lse -inf) takes no part, whatever its values hold
   const bool own = lt != -INFINITY;
+  Vec16 tv = {};
+  if (own) tv = reinterpret_cast<const Vec16*>(static_cast<const char*>(a.tail) + i * D * 2)[lane];
+  // the first 32 partials' states stay in registers for the second pass
+  int p0 = 0;
+  float2 x0 = make_float2(-INFINITY, 0.f);
+  if (lane < parts) {
+    p0 = at(lane);
+    x0 = a.ml[p0];
+  }
+  float m = x0.x;
+  for (int s = 32 + lane; s < parts; s += 32) m = fmaxf(m, a.ml[at(s)].x);
+  m = fmaxf(warp_max(m), lt);
+  if (m == -INFINITY) m = 0.f;
   const float wt = own ? exp2f(lt - m) : 0.f;
   float L = 0.f, o[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) o[k] = own ? wt * load_act(a.tail, i * D + V * lane + k, a.p.dtype) : 0.f;
+  for (int k = 0; k < V; k += 2) {
+    float2 f;
+    if constexpr (BF) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&tv.v[k / 2]));
+    else f = __half22float2(*reinterpret_cast<const __half2*>(&tv.v[k / 2]));
+    o[k] = own ? wt * f.x : 0.f;
+    o[k + 1] = own ? wt * f.y : 0.f;
+  }
   for (int s0 = 0; s0 < parts; s0 += 32) {
-    int64_t p = 0;
-    float w = 0.f;
-    if (s0 + lane < parts) {
-      p = at(s0 + lane);
-      const float2 x = a.ml[p];
-      w = exp2f(x.x - m);
-      L = fmaf(w, x.y, L);
+    int p = p0;
+    float2 x = x0;
+    if (s0 > 0) {
+      x = make_float2(-INFINITY, 0.f);
+      if (s0 + lane < parts) {
+        p = at(s0 + lane);
+        x = a.ml[p];
+      }
     }
+    const float w = exp2f(x.x - m);
+    L = fmaf(w, x.y, L);
     const int cnt = min(32, parts - s0);
     for (int s = 0; s < cnt; s += 8) {
       Vec v[8];
@@ -755,8 +821,10 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const PrefixArgs a)
   L = warp_sum(L) + wt;
   const bool any = L > 0.f || L != L;
   const float inv = any ? 1.f / L : 0.f;
+  Vec16 y;
 #pragma unroll
-  for (int k = 0; k < V; ++k) store_act(a.out, i * D + V * lane + k, o[k] * inv, a.p.dtype);
+  for (int k = 0; k < V; k += 2) y.v[k / 2] = pack16<BF>(o[k] * inv, o[k + 1] * inv);
+  reinterpret_cast<Vec16*>(static_cast<char*>(a.out) + i * D * 2)[lane] = y;
   if (a.lse && lane == 0) a.lse[i] = any ? (m + log2f(L)) * kLn2 : -INFINITY;
 }
 
@@ -805,31 +873,42 @@ int fma_splits(const carekv_prefix_t& p, int rows, int heads) {
   return std::max(1, std::min(want, (p.tokens + 127) / 128));
 }
 
-// Every CTA works on one SM for the whole launch.  Either the CTAs of a tile
-// share it evenly, or all CTAs share all units evenly and most of them cross
-// a tile's end, which costs about kCross units (the state of one tile written
-// out, the pipeline filled for the next).
-constexpr int kCross = 4;
+// Every CTA works on one SM for the whole launch.  With no more tiles than
+// SMs, either the CTAs of a tile share it evenly, or all CTAs share all units
+// evenly and most of them cross a tile's end, which costs about kCross units
+// (the state of one tile written out, the pipeline filled for the next).  A
+// tile of few units stays whole: the join is a launch of its own, as long as
+// about kJoin units.  With more tiles than SMs, each CTA takes as many whole
+// ones as all can have and a share of the rest.
+constexpr int kCross = 4, kJoin = 4;
 
 bool tc_split(const carekv_prefix_t& p, int rows, int heads, Split* s) {
   const int64_t per_head = static_cast<int64_t>(rows) * (heads / p.num_kv_heads);
   s->tile_rows = per_head <= kTcRows ? kTcRows : 2 * kTcRows;
   s->tiles = static_cast<int>((per_head + s->tile_rows - 1) / s->tile_rows);
-  s->blocks = (p.tokens + kTcBlock - 1) / kTcBlock;
+  s->blocks = static_cast<int>((static_cast<int64_t>(p.tokens) + kTcBlock - 1) / kTcBlock);
   const int64_t tiles = static_cast<int64_t>(s->tiles) * p.num_kv_heads, units = tiles * s->blocks;
   if (units > (1 << 30)) return false;
-  s->units = static_cast<int>(units);
   const int sms = sm_count();
-  const int per = static_cast<int>(std::min<int64_t>(tiles <= sms ? sms / tiles : 0, s->blocks));
-  const int64_t even = (units + sms - 1) / sms;
-  if (per > 0 && (s->blocks + per - 1) / per <= even + kCross) {
-    s->group = s->blocks;
-    s->per = per;
-    s->ctas = static_cast<int>(tiles) * per;
+  s->whole = 0;
+  s->ctas = sms;
+  if (tiles <= sms) {
+    const int per = s->blocks <= kJoin ? 1 : static_cast<int>(std::min<int64_t>(sms / tiles, s->blocks));
+    const int64_t even = (units + sms - 1) / sms;
+    if (per == 1 && s->blocks <= kJoin || (s->blocks + per - 1) / per <= even + kCross) {
+      s->group = s->blocks;
+      s->per = per;
+      s->ctas = static_cast<int>(tiles) * per;
+    } else {
+      s->group = static_cast<int>(units);
+      s->per = s->ctas = static_cast<int>(std::min<int64_t>(sms, units));
+    }
   } else {
-    s->group = s->units;
-    s->per = s->ctas = static_cast<int>(std::min<int64_t>(sms, units));
+    s->whole = static_cast<int>(tiles / sms);
+    s->group = static_cast<int>(tiles % sms) * s->blocks;   // may be 0: nothing is shared
+    s->per = sms;
   }
+  s->first = s->ctas * s->whole * s->blocks;
   s->base = s->group / s->per;
   s->rem = s->group % s->per;
   return true;
@@ -887,11 +966,12 @@ cudaError_t launch_tc(const PrefixArgs& a, const CUtensorMap& km, const CUtensor
                                    : launch_tc<D, BF, true>(a, km, vm, kh, vh, st);
 }
 
-// The join starts while the products' last CTAs run and waits for them itself.
+// The join of the shared tiles; it starts while the products' last CTAs run
+// and waits for them itself.
 cudaError_t launch_combine(const PrefixArgs& a, cudaStream_t st) {
-  const int64_t n = static_cast<int64_t>(a.rows) * a.heads;
+  const int tiles = a.sp.tiles * a.p.num_kv_heads - a.sp.ctas * a.sp.whole;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((n + 7) / 8));
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * (a.sp.tile_rows / 8)));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -899,8 +979,12 @@ cudaError_t launch_combine(const PrefixArgs& a, cudaStream_t st) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return a.p.head_dim == 128 ? cudaLaunchKernelEx(&cfg, prefix_combine_kernel<128>, a)
-                             : cudaLaunchKernelEx(&cfg, prefix_combine_kernel<64>, a);
+  const bool bf = a.p.dtype == CAREKV_BF16;
+  if (a.p.head_dim == 128)
+    return bf ? cudaLaunchKernelEx(&cfg, prefix_combine_kernel<128, true>, a)
+              : cudaLaunchKernelEx(&cfg, prefix_combine_kernel<128, false>, a);
+  return bf ? cudaLaunchKernelEx(&cfg, prefix_combine_kernel<64, true>, a)
+            : cudaLaunchKernelEx(&cfg, prefix_combine_kernel<64, false>, a);
 }
 
 }  // namespace
@@ -949,9 +1033,8 @@ cudaError_t launch_prefix(const carekv_prefix_t& p, const void* q, int64_t q_row
                                             : (bf ? launch_tc<64, true>(a, km, vm, kh, vh, st)
                                                   : launch_tc<64, false>(a, km, vm, kh, vh, st));
     if (e != cudaSuccess) return e;
-    // no tile is cut when every CTA starts on a tile
-    bool cut = false;
-    for (int c = 1; c < a.sp.ctas && !cut; ++c) cut = a.sp.start(c) % a.sp.blocks != 0;
+    // no tile is cut when every share starts on one
+    const bool cut = a.sp.group == a.sp.blocks ? a.sp.per > 1 : a.sp.rem != 0 || a.sp.base % a.sp.blocks != 0;
     return cut ? launch_combine(a, st) : cudaSuccess;
   }
   const int splits = p.tokens > 0 ? fma_splits(p, rows, heads) : 0;
