@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
     if (s.nb > 0) q_ready();
     for (;;) {
       const bool live = rho < total, warp_live = rho - lane < total;
-      const int vis = live ? visible(a, r) : 0;
+      const int vis = live ? visible(a, r) : a.p.tokens;   // rows past the last: whatever
       const int n_own = s.nb == 0 ? 0 : PAIR ? s.nb : (s.nb + 1 - st) >> 1;   // blocks of this stream
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n_own; ++j) {
@@ -581,31 +581,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
         ph ^= 1;
         tc_fence_after();
         const bool work = ok && warp_live;
-        uint32_t x[64];
+        // 32 columns at a time (128 scores would not fit the registers), the
+        // next 32 on their way: once for the maximum, once for the weights.
+        // The loops stay loops: the code is fetched anew by every launch, and
+        // its size shows in the first block's time.
+        uint32_t xa[32], xb[32];
         float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
         float mb = 0.f;
-        bool edge = false;
         const int t0 = (s.b0 + (PAIR ? j : 2 * j + st)) * kTcBlock;
-        auto fetch = [&](int c) {
-          tmem_ld64(ts + c, x);
+        const bool edge = work && __any_sync(0xffffffffu, t0 + kTcBlock > vis);
+        auto hide = [&](uint32_t (&x)[32], int c) {
           if (edge) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
+            for (int i = 0; i < 32; ++i)
               if (t0 + c + i >= vis) x[i] = 0xff800000u;
           }
         };
         if (work) {
-          // 64 columns at a time (128 scores would not fit the registers): the
-          // upper half for its maximum only, then the lower half, kept.  The
-          // loops over halves stay loops: the code is fetched anew by every
-          // launch, and its size shows in the first block's time.
-          edge = __any_sync(0xffffffffu, t0 + kTcBlock > vis);
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-          for (int c = 64; c >= 0; c -= 64) {
-            fetch(c);
+          auto maxima = [&](uint32_t (&x)[32], int c) {
+            hide(x, c);
 #pragma unroll
-            for (int i = 0; i < 64; ++i) mx[i & 3] = max_nan(mx[i & 3], __uint_as_float(x[i]));
+            for (int i = 0; i < 32; ++i) mx[i & 3] = max_nan(mx[i & 3], __uint_as_float(x[i]));
+          };
+          tmem_ld32_start(ts, xa);
+#pragma unroll 1
+          for (int c = 0; c < kTcBlock; c += 64) {
+            tmem_landed(xa);
+            tmem_ld32_start(ts + c + 32, xb);
+            maxima(xa, c);
+            tmem_landed(xb);
+            tmem_ld32_start(ts + (c + 64) % kTcBlock, xa);   // at the end: the first columns again
+            maxima(xb, c + 32);
           }
           float mt = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * a.scale2 - bias;
           if (mt == INFINITY) mt = __int_as_float(0x7fc00000);   // the row's weights are inf - inf
@@ -616,38 +623,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
             m = mn;
             l *= f;
             if (j > 0) {
+              tmem_landed(xa);
 #pragma unroll 1
               for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(to + c, o);
+                tmem_ld32(to + c, xb);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                tmem_st32(to + c, o);
+                for (int i = 0; i < 32; ++i) xb[i] = __float_as_uint(__uint_as_float(xb[i]) * f);
+                tmem_st32(to + c, xb);
               }
             }
           }
           mb = m == -INFINITY ? 0.f : -m;
         }
+        // weights of tokens c .. c + 31 to columns c / 2 .. of P, which lie
+        // over scores that are in registers or done by then
+        auto weights = [&](uint32_t (&x)[32], int c) {
+          hide(x, c);
+          const float2 sc = make_float2(a.scale2, a.scale2), mb2 = make_float2(mb, mb);
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 y = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc, mb2);
+            const float2 p = i % 8 < kFmaOf8 ? ex2_fma(y) : make_float2(ex2(y.x), ex2(y.y));
+            sum[i & 1] = add2(sum[i & 1], p);
+            w[i] = pack16<BF>(p.x, p.y);
+          }
+          tmem_st16(ts + c / 2, w);
+        };
 #pragma unroll 1
         for (int c = 0; c < kTcBlock; c += 64) {
           if (work) {
-            if (c > 0) fetch(c);
-            // weights of tokens c .. c + 63 to columns c / 2 .. of P, which
-            // lie over scores that are in registers or done by then
-            const float2 sc = make_float2(a.scale2, a.scale2), mb2 = make_float2(mb, mb);
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              uint32_t w[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 y = fma2(
-                    make_float2(__uint_as_float(x[32 * g + 2 * i]), __uint_as_float(x[32 * g + 2 * i + 1])), sc, mb2);
-                const float2 p = i % 8 < kFmaOf8 ? ex2_fma(y) : make_float2(ex2(y.x), ex2(y.y));
-                sum[i & 1] = add2(sum[i & 1], p);
-                w[i] = pack16<BF>(p.x, p.y);
-              }
-              tmem_st16(ts + c / 2 + 16 * g, w);
-            }
+            tmem_landed(xa);
+            tmem_ld32_start(ts + c + 32, xb);
+            weights(xa, c);
+            tmem_landed(xb);
+            if (c == 0) tmem_ld32_start(ts + 64, xa);
+            weights(xb, c + 32);
             tmem_wait_st();
           }
           tc_fence_before();

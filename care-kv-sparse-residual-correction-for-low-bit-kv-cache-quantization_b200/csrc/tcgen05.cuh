@@ -37,16 +37,21 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld64(uint32_t addr, uint32_t (&r)[64]) {
+// The same in two steps: the load starts, and tmem_landed waits for all loads
+// of the thread; the registers pass through the wait, so no use of them can
+// be moved before it.
+__device__ __forceinline__ void tmem_ld32_start(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,"
-      "%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : CAREKV_R8(r, 0), CAREKV_R8(r, 8), CAREKV_R8(r, 16), CAREKV_R8(r, 24), CAREKV_R8(r, 32), CAREKV_R8(r, 40),
-        CAREKV_R8(r, 48), CAREKV_R8(r, 56)
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : CAREKV_R8(r, 0), CAREKV_R8(r, 8), CAREKV_R8(r, 16), CAREKV_R8(r, 24)
       : "r"(addr)
       : "memory");
+}
+#define CAREKV_P8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
+__device__ __forceinline__ void tmem_landed(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : CAREKV_P8(r, 0), CAREKV_P8(r, 8), CAREKV_P8(r, 16), CAREKV_P8(r, 24)::"memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile(
