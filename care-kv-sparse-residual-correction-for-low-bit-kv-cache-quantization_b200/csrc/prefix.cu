@@ -148,9 +148,11 @@ __global__ void __launch_bounds__(kFmaRows * 32) prefix_fma_kernel(const PrefixA
 // ulp per weight, independent between tokens, like the result's own rounding.
 constexpr int kTcThreads = 320, kTcRows = 128, kTcBlock = 128;
 constexpr float kRaise = 8.f;
-// Of 8 pairs of weights, those computed on the FMA pipe: the 16 special-function
-// lanes of an SM would take 2048 cycles for a block's 256 rows x 128 weights.
-constexpr int kFmaOf8 = 3;
+// One of so many pairs of weights is computed on the FMA pipe: the 16
+// special-function lanes of an SM take 2048 cycles for a block's 256 rows x
+// 128 weights, half of what the block takes (512 rows x 8 heads of 64 on 8192
+// tokens: 86 us without, 81 with every fourth, 84 with three of eight).
+constexpr int kFmaEvery = 4;
 
 template <int D, bool PAIR>
 struct TcLayout {
@@ -640,13 +642,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
         auto weights = [&](uint32_t (&x)[32], int c) {
           hide(x, c);
           const float2 sc = make_float2(a.scale2, a.scale2), mb2 = make_float2(mb, mb);
+          float2 p[16];
           uint32_t w[16];
 #pragma unroll
+          for (int i = 0; i < 16; ++i)
+            p[i] = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc, mb2);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i % kFmaEvery != 0) p[i] = make_float2(ex2(p[i].x), ex2(p[i].y));
+#pragma unroll
+          for (int i = 0; i < 16; i += kFmaEvery) p[i] = ex2_fma(p[i]);
+#pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float2 y = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc, mb2);
-            const float2 p = i % 8 < kFmaOf8 ? ex2_fma(y) : make_float2(ex2(y.x), ex2(y.y));
-            sum[i & 1] = add2(sum[i & 1], p);
-            w[i] = pack16<BF>(p.x, p.y);
+            sum[i & 1] = add2(sum[i & 1], p[i]);
+            w[i] = pack16<BF>(p[i].x, p[i].y);
           }
           tmem_st16(ts + c / 2, w);
         };
