@@ -339,6 +339,14 @@ int carekv_decode_attention_shard(const carekv_config_t* cfg, const carekv_cache
                                   int32_t max_pages_used, const carekv_route_params_t* params,
                                   const float* sketch_proj, void* workspace, size_t workspace_bytes_,
                                   const carekv_shard_t* shard, void* stream) {
+  return carekv_decode_attention_lse(cfg, cache, layer, q, out, nullptr, dtype, seq_begin, seq_count, max_pages_used,
+                                     params, sketch_proj, workspace, workspace_bytes_, shard, stream);
+}
+
+int carekv_decode_attention_lse(const carekv_config_t* cfg, const carekv_cache_t* cache, int32_t layer, const void* q,
+                                void* out, float* lse, int32_t dtype, int32_t seq_begin, int32_t seq_count,
+                                int32_t max_pages_used, const carekv_route_params_t* params, const float* sketch_proj,
+                                void* workspace, size_t workspace_bytes_, const carekv_shard_t* shard, void* stream) {
   CHECK(validate_config(cfg));
   CHECK(validate_shard(cfg, shard));
   CHECK(validate_cache(cfg, cache));
@@ -361,7 +369,8 @@ int carekv_decode_attention_shard(const carekv_config_t* cfg, const carekv_cache
   const int64_t off = static_cast<int64_t>(shard->kvh_begin) * qn * cfg->head_dim * act_bytes(dtype);
   return decode_attention(*cfg, *cache, layer, static_cast<const char*>(q) + off, static_cast<char*>(out) + off, dtype,
                           seq_begin, seq_count, std::max(1, max_pages_used), *params, workspace, workspace_bytes_,
-                          sketch_proj, shard->kvh_total * qn, as_stream(stream));
+                          sketch_proj, shard->kvh_total * qn,
+                          lse ? lse + static_cast<int64_t>(shard->kvh_begin) * qn : nullptr, as_stream(stream));
 }
 
 int carekv_prefill_workspace_bytes(const carekv_config_t* cfg, int32_t n_pos, int32_t max_pages_used,

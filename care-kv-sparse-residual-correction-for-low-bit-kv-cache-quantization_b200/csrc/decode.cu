@@ -245,7 +245,7 @@ int decode_attention_chunks(int seq_count) {
 int decode_attention(const carekv_config_t& cfg, const carekv_cache_t& cache, int layer, const void* q,
                      void* out, int dtype, int seq_begin, int seq_count, int p_used,
                      const carekv_route_params_t& rp, void* ws, size_t ws_bytes, const float* sketch_proj,
-                     int act_heads, cudaStream_t st) {
+                     int act_heads, float* lse, cudaStream_t st) {
   if (ws_bytes < workspace_bytes(cfg, seq_count, p_used)) return CAREKV_ERR_WORKSPACE;
   DecodeArgs a;
   a.cfg = cfg;
@@ -303,6 +303,7 @@ int decode_attention(const carekv_config_t& cfg, const carekv_cache_t& cache, in
   a.o_exact = nullptr;
   a.v_rows = nullptr;
   a.v_pnorm = nullptr;
+  a.lse = lse;
   if (a.qn != 1 && a.qn != 2 && a.qn != 4 && a.qn != 8) return CAREKV_ERR_UNSUPPORTED;
 
   const int per = chunk_size(seq_count);
@@ -321,6 +322,7 @@ int decode_attention(const carekv_config_t& cfg, const carekv_cache_t& cache, in
     ac.seq_begin = seq_begin + s0;
     ac.q = static_cast<const char*>(q) + static_cast<int64_t>(s0) * act_heads * D * es;
     ac.out = static_cast<char*>(out) + static_cast<int64_t>(s0) * act_heads * D * es;
+    if (lse) ac.lse = lse + static_cast<int64_t>(s0) * act_heads;
     ac.sel_out = a.sel_out + bh0 * qn * a.sel_stride;
     ac.scores = a.scores + bh0 * qn * NGs;
     ac.S = a.S + bh0 * qn * p_used * kPage;

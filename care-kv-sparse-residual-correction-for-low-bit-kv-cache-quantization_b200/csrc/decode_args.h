@@ -48,6 +48,7 @@ struct DecodeArgs {
   const float* o_exact;  // [bh][qn][D] sum_t A V for the exact form (prefill), or null
   const float* v_rows;   // [H][p_used*16][D] or null
   const float* v_pnorm;  // [H][p_used] Frobenius norm of each page's rows, or null
+  float* lse;            // decode: [row][act_heads] log-sum-exp of the corrected attention, or null
 };
 
 // Position of token t (0..15) inside a page's 16 logits: the narrow pass

@@ -47,7 +47,7 @@ cudaError_t launch_decode_generic(DecodeArgs& a, cudaStream_t st, int n_bh);
 int decode_attention(const carekv_config_t& cfg, const carekv_cache_t& cache, int layer, const void* q,
                      void* out, int dtype, int seq_begin, int seq_count, int p_used,
                      const carekv_route_params_t& rp, void* ws, size_t ws_bytes, const float* sketch_proj,
-                     int act_heads, cudaStream_t st);
+                     int act_heads, float* lse, cudaStream_t st);
 size_t workspace_bytes(const carekv_config_t& c, int seq_count, int p_used);
 void prepare_decode_streams();               // creates the chunk streams of the current device (not under capture)
 int decode_attention_chunks(int seq_count);   // batch chunks one decode attention call runs

@@ -340,6 +340,9 @@ __device__ __forceinline__ void route_body(const DecodeArgs& a, int bh, RouteSme
       const int i = idx / D, c = idx % D;
       store_act(a.out, (static_cast<int64_t>(s) * Hq + h * QG + q0 + i) * D + c, sm.O[i][c], a.dt);
     }
+    // log sum of the tail's exponentials (attention states are merged by it)
+    if (!PF && a.lse != nullptr && tid < QN)
+      a.lse[static_cast<int64_t>(s) * Hq + h * QG + q0 + tid] = sm.L[tid] > 0.f ? sm.M[tid] + logf(sm.L[tid]) : -INFINITY;
   };
   if (np == 0 || rp.kind == CAREKV_KIND_NONE) {
     write_base();
@@ -1724,14 +1727,20 @@ __device__ __forceinline__ void route_body(const DecodeArgs& a, int bh, RouteSme
       const float oe = o_exact ? o_exact[row * D + tid] : ob;
       const float as = (po_direct && a.pl) ? a.pl[row] : 1.f;
       float delta;
+      float norm = 1.f;   // new normaliser over the old one, times e^-mshift
       if (ill) {
         // direct form: (cbase sum_notS A V + sum_S A cbase e^ds V) / (cbase sum_notS A + sum_S A cbase e^ds)
         float on = 0.f, zn = 0.f;
         for (int w = 0; w < NW; ++w) { on += sm.acc2[w][tid]; zn += sm.z2[w]; }
-        delta = __fdiv_rn(fmaf(cbase, on, n), fmaf(cbase, zn, z)) - ob;
+        norm = fmaf(cbase, zn, z);
+        delta = __fdiv_rn(fmaf(cbase, on, n), norm) - ob;
       } else {
-        delta = exact ? (__fdiv_rn(fmaf(cbase, oe, n), fmaf(cbase, as, z)) - ob) : (n - z * ob);
+        if (exact) norm = fmaf(cbase, as, z);
+        delta = exact ? (__fdiv_rn(fmaf(cbase, oe, n), norm) - ob) : (n - z * ob);
       }
+      // the linear form keeps the base normaliser
+      if (!PF && a.lse != nullptr && tid == 0)
+        a.lse[static_cast<int64_t>(s) * Hq + h * QG + q0 + i] = sm.M[i] + logf(sm.L[i]) + mshift + logf(norm);
       store_act(a.out, (static_cast<int64_t>(s) * Hq + h * QG + q0 + i) * D + tid, ob + delta, a.dt);
     }
     __syncthreads();

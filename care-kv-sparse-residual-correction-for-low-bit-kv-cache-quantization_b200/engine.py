@@ -19,6 +19,7 @@ import torch
 from . import _lib
 from .cache import CAREKVCache
 from .config import legacy_router, resolve_route_params, resolve_store_params
+from .prefix import SharedPrefix
 
 
 def decode_router(router: Optional[str] = None) -> str:
@@ -149,12 +150,18 @@ class DecodeEngine:
 
     def attend(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None, seq_begin: int = 0,
                kind: Optional[str] = None, correction: bool = True, score_normalize=None, k_corr_scale=None,
-               pages: Optional[int] = None, router: Optional[str] = None) -> torch.Tensor:
+               pages: Optional[int] = None, router: Optional[str] = None, prefix: Optional[SharedPrefix] = None,
+               return_lse: bool = False):
         """Decode attention for [seq_count, Hq, D] queries against the cache.
         router: "vectorized" (vectorized_joint_correction per kv head, the
         default) or "cached" (the reference decode step's ResidualRouter.route
         + apply_slot_corrections per query head); None reads
-        CAREKV_DECODE_ROUTER."""
+        CAREKV_DECODE_ROUTER.
+        prefix: tokens shared by all sequences, before their own: the cache's
+        result (its residual correction routed over the own tokens alone) is
+        merged with attention over the prefix of this layer (same dtype and
+        kv heads as the cache's).
+        return_lse: also the fp32 log-sum-exp [seq_count, Hq] of the attention."""
         cfg = self.cfg
         n = q.shape[0]
         q = self._check_tensor(q, (n, self.kvh_total * self.qn, cfg.head_dim), "decode q")
@@ -168,11 +175,23 @@ class DecodeEngine:
             rp.kind = _lib.KIND_NONE
         nbytes = self.workspace_bytes(n, pages)
         ws = self.workspace(nbytes)
-        _lib.check(_lib.lib().carekv_decode_attention_shard(
-            ctypes.byref(self.cache.ccfg), ctypes.byref(self.cache.c), layer, q.data_ptr(), out.data_ptr(),
-            _DT[q.dtype], seq_begin, n, pages, ctypes.byref(rp), self._sketch_ptr(), ws.data_ptr(), ws.numel(),
-            ctypes.byref(self.shard), self._stream()), "carekv_decode_attention")
-        return out
+        lse = None
+        if return_lse or prefix is not None:
+            lse = torch.full((n, q.shape[1]), float("-inf"), dtype=torch.float32, device=q.device)
+        own = out if prefix is None else torch.empty_like(q)
+        _lib.check(_lib.lib().carekv_decode_attention_lse(
+            ctypes.byref(self.cache.ccfg), ctypes.byref(self.cache.c), layer, q.data_ptr(), own.data_ptr(),
+            None if lse is None else lse.data_ptr(), _DT[q.dtype], seq_begin, n, pages, ctypes.byref(rp),
+            self._sketch_ptr(), ws.data_ptr(), ws.numel(), ctypes.byref(self.shard), self._stream()),
+            "carekv_decode_attention")
+        if prefix is not None:
+            h0, h1 = self.shard.kvh_begin * self.qn, (self.shard.kvh_begin + cfg.num_kv_heads) * self.qn
+            if h1 - h0 == q.shape[1]:
+                _, lse = prefix.attend(layer, q, tail=(own, lse), out=out, return_lse=True)
+            else:
+                out[:, h0:h1], lse[:, h0:h1] = prefix.attend(layer, q[:, h0:h1], tail=(own[:, h0:h1], lse[:, h0:h1]),
+                                                             return_lse=True)
+        return (out, lse) if return_lse else out
 
     def prefill_correct(self, layer: int, seq: int, q: torch.Tensor, attn: torch.Tensor, o_base: torch.Tensor,
                         o_exact: Optional[torch.Tensor] = None, attn_sum: Optional[torch.Tensor] = None,

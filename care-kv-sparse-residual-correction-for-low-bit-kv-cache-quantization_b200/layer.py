@@ -37,7 +37,10 @@ from torch import Tensor, nn
 from .cache import CAREKVCache
 from .config import CacheConfig, any_read_budget
 from .engine import DecodeEngine
+from .prefix import SharedPrefix
 from .quantizer import QuantConfig, dequantize, quantize
+from .rotary import RotaryEmbedding
+from .weights import PackedWeight
 
 try:  # RoPE as the reference applies it (layer.py:66)
     from transformers.models.llama.modeling_llama import apply_rotary_pos_emb
@@ -76,10 +79,11 @@ def _rope(q: Tensor, k: Tensor, position_embeddings) -> Tuple[Tensor, Tensor]:
     return apply_rotary_pos_emb(q, k, cos, sin)
 
 
-def causal_attention(Q: Tensor, K: Tensor, V: Tensor, attention_mask: Optional[Tensor]) -> Tensor:
+def causal_attention(Q: Tensor, K: Tensor, V: Tensor, attention_mask: Optional[Tensor], return_lse: bool = False):
     """O = softmax(Q K^T / sqrt(D) + mask) V with scores and softmax in fp32
     (layer.py:936-973).  Q [B, Hq, T, D], K / V [B, Hq, T, D]; the additive
-    mask is [T, T] or broadcastable to [B, 1, T, T]; None -> causal."""
+    mask is [T, T] or broadcastable to [B, 1, T, T]; None -> causal.
+    return_lse: also the fp32 log-sum-exp of the scores [B, Hq, T]."""
     D = Q.shape[-1]
     T = Q.shape[-2]
     scores = torch.matmul(Q.float(), K.float().transpose(-1, -2)) / math.sqrt(D)
@@ -94,11 +98,17 @@ def causal_attention(Q: Tensor, K: Tensor, V: Tensor, attention_mask: Optional[T
         causal = torch.full((T, T), torch.finfo(scores.dtype).min, device=scores.device, dtype=scores.dtype)
         scores = scores + torch.triu(causal, diagonal=1)
     w = torch.softmax(scores, dim=-1, dtype=torch.float32).to(Q.dtype)
-    return torch.matmul(w, V)
+    O = torch.matmul(w, V)
+    return (O, torch.logsumexp(scores, dim=-1)) if return_lse else O
 
 
 class CAREKVLayer(nn.Module):
-    """Drop-in attention layer (layer.py:147-179): projections + CARE-KV cache."""
+    """Drop-in attention layer (layer.py:147-179): projections + CARE-KV cache.
+
+    quantize_weights() turns the projections into 4-bit weights; with `rotary`
+    set (a RotaryEmbedding) the calls take integer `positions` in place of
+    cos / sin tables; `prefix` (a SharedPrefix) puts the same prompt, held
+    once, before every sequence's own tokens."""
 
     def __init__(self, cfg: CacheConfig, layer_id: int, W_Q: Tensor, W_K: Tensor, W_V: Tensor, W_O: Tensor,
                  device: torch.device = torch.device("cpu")):
@@ -111,6 +121,22 @@ class CAREKVLayer(nn.Module):
         self.W_V = nn.Parameter(W_V, requires_grad=False)
         self.W_O = nn.Parameter(W_O, requires_grad=False)
         self.base_qcfg = QuantConfig(bits=cfg.base_bits, group_size=cfg.group_size)
+        self.rotary: Optional[RotaryEmbedding] = None
+        self._packed: Dict[str, PackedWeight] = {}
+
+    def quantize_weights(self, group_size: int = 32) -> "CAREKVLayer":
+        """Replace the projections by 4-bit weights with one scale per
+        `group_size` input channels (the package quantizer's codes)."""
+        for name in ("W_Q", "W_K", "W_V", "W_O"):
+            if name not in self._packed:
+                self._packed[name] = PackedWeight.from_dense(getattr(self, name).data, group_size)
+                setattr(self, name, None)
+        return self
+
+    def _linear(self, name: str, x: Tensor) -> Tensor:
+        """x [..., K] @ W^T with the dense or the 4-bit weight."""
+        w = self._packed.get(name)
+        return x @ getattr(self, name).T if w is None else w.matmul(x)
 
     # ── projections ──────────────────────────────────────────────────
     def _project(self, hidden: Tensor):
@@ -118,34 +144,52 @@ class CAREKVLayer(nn.Module):
         cfg = self.cfg
         B, T, _ = hidden.shape
         Hq, Hkv, D = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
-        q = (hidden @ self.W_Q.T).reshape(B, T, Hq, D).transpose(1, 2)
-        k = (hidden @ self.W_K.T).reshape(B, T, Hkv, D).transpose(1, 2)
-        v = (hidden @ self.W_V.T).reshape(B, T, Hkv, D).transpose(1, 2)
+        q = self._linear("W_Q", hidden).reshape(B, T, Hq, D).transpose(1, 2)
+        k = self._linear("W_K", hidden).reshape(B, T, Hkv, D).transpose(1, 2)
+        v = self._linear("W_V", hidden).reshape(B, T, Hkv, D).transpose(1, 2)
         return q, k, v
+
+    def _rotate(self, q: Tensor, k: Tensor, position_embeddings, positions: Optional[Tensor]):
+        """q [B, Hq, T, D], k [B, Hkv, T, D] -> post-RoPE, contiguous where the
+        rotary kernel wrote them."""
+        if positions is None:
+            return _rope(q, k, position_embeddings)
+        if self.rotary is None:
+            raise ValueError("positions need layer.rotary (a RotaryEmbedding)")
+        if position_embeddings is not None:
+            raise ValueError("position_embeddings or positions, not both")
+        yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
+        self.rotary(q.transpose(1, 2), k.transpose(1, 2), positions,
+                    out=(yq.transpose(1, 2), yk.transpose(1, 2)))
+        return yq, yk
 
     def _out(self, O: Tensor) -> Tensor:
         """O [B, Hq, T, D] -> [B, T, dm]."""
         B, Hq, T, D = O.shape
-        return O.transpose(1, 2).reshape(B, T, Hq * D) @ self.W_O.T
+        return self._linear("W_O", O.transpose(1, 2).reshape(B, T, Hq * D))
 
     # ── prefill ──────────────────────────────────────────────────────
     def prefill(self, cache: CAREKVCache, hidden: Tensor, sink_tokens: int = 4,
                 attention_mask: Optional[Tensor] = None,
                 position_embeddings: Optional[Tuple[Tensor, Tensor]] = None,
-                token_start_abs: int = 0, debug_stats: Optional[Dict[str, Any]] = None, seq: int = 0) -> Tensor:
+                token_start_abs: int = 0, debug_stats: Optional[Dict[str, Any]] = None, seq: int = 0,
+                positions: Optional[Tensor] = None, prefix: Optional[SharedPrefix] = None) -> Tensor:
         """hidden [T, dm] of sequence `seq` -> attention output [T, dm] (layer.py:643-845)."""
         pe = None
         if position_embeddings is not None:
             cos, sin = position_embeddings
             pe = (cos if cos.dim() == 3 else cos.unsqueeze(0), sin if sin.dim() == 3 else sin.unsqueeze(0))
         return self.prefill_batch(cache, hidden.unsqueeze(0), sink_tokens, attention_mask, pe,
-                                  token_start_abs, seq_begin=seq)[0]
+                                  token_start_abs, seq_begin=seq, positions=positions, prefix=prefix)[0]
 
     def prefill_batch(self, cache: CAREKVCache, hidden: Tensor, sink_tokens: int = 4,
                       attention_mask: Optional[Tensor] = None,
                       position_embeddings: Optional[Tuple[Tensor, Tensor]] = None,
-                      token_start_abs: int = 0, seq_begin: int = 0) -> Tensor:
-        """hidden [B, T, dm] of sequences seq_begin .. seq_begin+B -> [B, T, dm]."""
+                      token_start_abs: int = 0, seq_begin: int = 0, positions: Optional[Tensor] = None,
+                      prefix: Optional[SharedPrefix] = None) -> Tensor:
+        """hidden [B, T, dm] of sequences seq_begin .. seq_begin+B -> [B, T, dm].
+        positions [T] or [B, T]; with a prefix of N tokens the own tokens stand
+        at N onwards and attend over it too (only they enter the cache)."""
         mode = resolve_prefill_mode()
         if mode == "carekv_eval":
             raise NotImplementedError(
@@ -154,10 +198,13 @@ class CAREKVLayer(nn.Module):
         if mode not in ("fp", "base_quant", "carekv_stored"):
             raise ValueError(f"Unknown CAREKV_PREFILL_MODE={mode}")
         cfg = self.cfg
+        if prefix is not None and mode == "carekv_stored" and any_read_budget(cfg):
+            raise NotImplementedError("CAREKV_PREFILL_MODE=carekv_stored: the stored-slot prefill correction knows no "
+                                      "shared prefix; use fp or base_quant")
         B, T, _ = hidden.shape
         g = cfg.num_heads // cfg.num_kv_heads
         q, k, v = self._project(hidden)
-        q_post, k_post = _rope(q, k, position_embeddings)
+        q_post, k_post = self._rotate(q, k, position_embeddings, positions)
         eng = engine_for(cache)
         eng.prefill_store(self.layer_id, k_post.contiguous(), v.contiguous(), seq_begin=seq_begin,
                           token_start=token_start_abs, sink_tokens=sink_tokens)
@@ -171,8 +218,13 @@ class CAREKVLayer(nn.Module):
         if g > 1:
             K_att = K_att.repeat_interleave(g, dim=1)
             V_att = V_att.repeat_interleave(g, dim=1)
-        O = causal_attention(q_post, K_att, V_att, attention_mask)
-        return self._out(O)
+        if prefix is None:
+            return self._out(causal_attention(q_post, K_att, V_att, attention_mask))
+        O, lse = causal_attention(q_post, K_att, V_att, attention_mask, return_lse=True)
+        Hq, D = cfg.num_heads, cfg.head_dim
+        rows = lambda x: x.transpose(1, 2).reshape(B * T, Hq, *x.shape[3:])    # noqa: E731
+        O = prefix.attend(self.layer_id, rows(q_post), tail=(rows(O), rows(lse)))
+        return self._linear("W_O", O.reshape(B, T, Hq * D))
 
     def _stored_correction(self, eng: DecodeEngine, q: Tensor, K_hat: Tensor, V_hat: Tensor,
                            attention_mask: Optional[Tensor], seq_begin: int, chunk: int = 256) -> Tensor:
@@ -262,14 +314,17 @@ class CAREKVLayer(nn.Module):
     # ── decode ───────────────────────────────────────────────────────
     def decode_step(self, cache: CAREKVCache, hidden: Tensor,
                     position_embeddings: Optional[Tuple[Tensor, Tensor]] = None,
-                    debug_stats: Optional[Dict[str, Any]] = None, seq: int = 0) -> Tensor:
+                    debug_stats: Optional[Dict[str, Any]] = None, seq: int = 0,
+                    positions: Optional[Tensor] = None, prefix: Optional[SharedPrefix] = None) -> Tensor:
         """hidden [1, dm] of sequence `seq` -> [1, dm] (layer.py:978-1163)."""
-        return self.decode_step_batch(cache, hidden.reshape(1, -1), position_embeddings, seq_begin=seq)
+        return self.decode_step_batch(cache, hidden.reshape(1, -1), position_embeddings, seq_begin=seq,
+                                      positions=positions, prefix=prefix)
 
     def decode_step_batch(self, cache: CAREKVCache, hidden: Tensor,
                           position_embeddings: Optional[Tuple[Tensor, Tensor]] = None,
-                          seq_begin: int = 0) -> Tensor:
-        """hidden [B, dm] (one new token per sequence) -> [B, dm].
+                          seq_begin: int = 0, positions: Optional[Tensor] = None,
+                          prefix: Optional[SharedPrefix] = None) -> Tensor:
+        """hidden [B, dm] (one new token per sequence) -> [B, dm]; positions [B].
 
         Appends the token's K / V (quantize, pack; the page-full residual store
         when a page completes) and runs decode attention with the residual
@@ -288,8 +343,8 @@ class CAREKVLayer(nn.Module):
             if cos.shape[0] == 1 and B > 1:
                 cos, sin = cos.expand(B, 1, -1), sin.expand(B, 1, -1)
             pe = (cos, sin)
-        q_post, k_post = _rope(q, k, pe)
+        q_post, k_post = self._rotate(q, k, pe, None if positions is None else positions.reshape(B, 1))
         eng = engine_for(cache)
         eng.append(self.layer_id, k_post[:, :, 0].contiguous(), v[:, :, 0].contiguous(), seq_begin=seq_begin)
-        O = eng.attend(self.layer_id, q_post[:, :, 0].contiguous(), seq_begin=seq_begin)   # [B, Hq, D]
-        return O.reshape(B, cfg.num_heads * cfg.head_dim) @ self.W_O.T
+        O = eng.attend(self.layer_id, q_post[:, :, 0].contiguous(), seq_begin=seq_begin, prefix=prefix)   # [B, Hq, D]
+        return self._linear("W_O", O.reshape(B, cfg.num_heads * cfg.head_dim))

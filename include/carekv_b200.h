@@ -318,6 +318,20 @@ int carekv_decode_attention_shard(const carekv_config_t *cfg, const carekv_cache
                                   void *workspace, size_t workspace_bytes, const carekv_shard_t *shard,
                                   void *stream);
 
+/* carekv_decode_attention_shard that also writes lse [seq_count]
+ * [shard->kvh_total * QN] fp32 (NULL: not wanted; only the shard's heads are
+ * written): the natural log of the sum of the row's attention weights before
+ * normalisation, e^(logit), or e^(logit + ds) under the exact K correction
+ * (the linear one leaves the base sum); -inf for an empty sequence.  With it
+ * the result can be merged with attention over other tokens
+ * (carekv_prefix_attention). */
+int carekv_decode_attention_lse(const carekv_config_t *cfg, const carekv_cache_t *cache, int32_t layer,
+                                const void *q, void *out, float *lse, int32_t dtype, int32_t seq_begin,
+                                int32_t seq_count, int32_t max_pages_used,
+                                const carekv_route_params_t *params, const float *sketch_proj,
+                                void *workspace, size_t workspace_bytes, const carekv_shard_t *shard,
+                                void *stream);
+
 /* Kernel launches one carekv_decode_attention call over `seq_count`
  * sequences issues: a split-K pass and a route kernel per batch chunk.  The
  * batch runs in CAREKV_ATTEND_CHUNKS (environment, 1 / 2 / 4, default 1)

@@ -1,0 +1,252 @@
+"""The cache's decode attention with its log-sum-exp, merged with a shared
+prefix, and a layer step that runs 4-bit projections, rotary positions and the
+prefix together (GPU)."""
+
+import math
+import zlib
+
+import numpy as np
+import pytest
+import torch
+
+import oracle
+from conftest import load_pkg
+from helpers import PAPER_BEST_ENV, env, oracle_cache_for, oracle_selection, route_cfg_from
+
+pytestmark = pytest.mark.gpu
+
+TDT = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+# attention outputs: the decode path's own tolerances (test_gpu_decode.py)
+TOL = {"fp32": (1e-3, 2e-3), "fp16": (3e-3, 3e-3), "bf16": (1e-2, 1e-2)}
+# a log-sum-exp moves by at most the largest error of a logit; fp32 logits of
+# D products of up to ~60 x 4 are off by D 2^-24 240 < 2e-3
+LSE_TOL = 2e-3
+
+
+@pytest.fixture(scope="module")
+def pkg():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    return load_pkg()
+
+
+def build(pkg, D, bits, g, Hq, Hkv, dt, lens, seed, **kw):
+    cfg = pkg.CacheConfig(num_layers=1, num_heads=Hq, num_kv_heads=Hkv, head_dim=D, page_size=16,
+                          max_pages=max(lens) // 16 + 3, base_bits=bits, group_size=g, scale_quant="int8",
+                          packed_base=True, store_budget_mode="absolute", store_abs_k=2, store_abs_v=2,
+                          route_policy="joint", store_sketch=False, **kw)
+    cache = pkg.CAREKVCache(cfg, torch.device("cuda"), batch=len(lens))
+    eng = pkg.DecodeEngine(cache)
+    rng = np.random.default_rng(seed)
+    seqs = []
+    for b, T in enumerate(lens):
+        oc = oracle_cache_for(cfg)
+        if T:
+            K = rng.standard_normal((Hkv, T, D)).astype(np.float32)
+            K[:, :, :4] *= 20.0
+            V = rng.standard_normal((Hkv, T, D)).astype(np.float32)
+            K, V = oracle.round_to(K, dt), oracle.round_to(V, dt)
+            eng.prefill_store(0, torch.from_numpy(K).cuda().to(TDT[dt])[None],
+                              torch.from_numpy(V).cuda().to(TDT[dt])[None], seq_begin=b)
+            for h in range(Hkv):
+                oc.prefill_write(0, h, K[h], V[h], dt)
+        seqs.append(oc)
+    q = oracle.round_to(rng.standard_normal((len(lens), Hq, D)).astype(np.float32), dt)
+    return cfg, cache, eng, seqs, q
+
+
+CASES = [
+    # name, D, bits, g, Hq, Hkv, dt, lengths, correction mode or None (no correction)
+    ("base_mha", 128, 3, 32, 4, 4, "fp32", (90, 17, 0), None),
+    ("exact_mha", 128, 3, 32, 4, 4, "fp32", (150, 33, 0), "exact"),
+    ("exact_gqa4_int2", 128, 2, 32, 8, 2, "fp32", (64, 40), "exact"),
+    ("exact_gqa8_d64", 64, 3, 32, 16, 2, "fp16", (77, 130), "exact"),
+    ("linear_gqa2_int4", 64, 4, 64, 4, 2, "fp32", (50, 96), "linear"),
+    ("exact_bf16", 128, 3, 32, 4, 4, "bf16", (100, 64), "exact"),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=[c[0] for c in CASES])
+def test_log_sum_exp_matches_oracle(pkg, case):
+    """lse = log sum e^(logit), e^(logit + ds) under the exact correction; -inf for an empty sequence."""
+    name, D, bits, g, Hq, Hkv, dt, lens, mode = case
+    grp = Hq // Hkv
+    with env(**dict(PAPER_BEST_ENV, CAREKV_K_CORRECTION_MODE=mode or "exact")):
+        cfg, cache, eng, seqs, q = build(pkg, D, bits, g, Hq, Hkv, dt, lens, zlib.crc32(name.encode()),
+                                         read_budget_mode="absolute", read_abs_k=2, read_abs_v=2)
+        qt = torch.from_numpy(q).cuda().to(TDT[dt])
+        plain = eng.attend(0, qt, correction=mode is not None)
+        out, lse = eng.attend(0, qt, correction=mode is not None, return_lse=True)
+        assert torch.equal(out, plain)       # asking for it changes nothing
+        pages = max(eng._pages(b, 0) for b in range(len(lens)))
+        sel = eng.last_selection(0, 0, len(lens), pages) if mode else None
+        rc = route_cfg_from(cfg)
+        lse = lse.double().cpu().numpy()
+        checked = 0
+        for b, oc in enumerate(seqs):
+            for h in range(Hkv):
+                rows = slice(h * grp, (h + 1) * grp)
+                if lens[b] == 0:
+                    assert np.all(np.isneginf(lse[b, rows]))
+                    continue
+                _, info = oracle.decode_attention_kvh(oc, 0, h, q[b, rows], rc, correction=mode is not None)
+                S = info["S"].astype(np.float64)
+                if mode == "exact":
+                    want_sel = oracle_selection(info, grp)
+                    for si, e in enumerate(info["k_index"]):
+                        c0 = e["cg"] * cfg.k_channel_group
+                        ds = q[b, rows][:, c0:c0 + cfg.k_channel_group].astype(np.float64) @ e["R"].T / math.sqrt(D)
+                        S[:, e["pstart"]:e["pstart"] + e["nvalid"]] += info["sel_k"][:, si, None] * ds
+                for i in range(grp):
+                    if mode == "exact" and sorted(sel[(b, h, i)]) != want_sel[i]:
+                        continue     # a tie within rounding: another, equally good set of slots
+                    m = S[i].max()
+                    want = m + math.log(np.exp(S[i] - m).sum())
+                    assert abs(lse[b, h * grp + i] - want) <= LSE_TOL + 1e-5 * abs(want), (b, h, i)
+                    checked += 1
+        assert checked >= 0.9 * Hq * sum(1 for n in lens if n)
+        cache.check_errors()
+
+
+@pytest.mark.parametrize("dt,D,Hq,Hkv", [("fp32", 128, 8, 2), ("fp16", 64, 16, 2), ("bf16", 128, 4, 4)])
+def test_prefix_and_cache_equal_one_softmax(pkg, dt, D, Hq, Hkv):
+    """attend(prefix=...) = one softmax over the prefix's and the cache's (dequantized) tokens."""
+    with env(**PAPER_BEST_ENV):
+        lens = (70, 5, 0, 33)
+        cfg, cache, eng, seqs, q = build(pkg, D, 3, 32, Hq, Hkv, dt, lens, 7, read_budget_mode="absolute",
+                                         read_abs_k=0, read_abs_v=0)
+        N, grp = 300, Hq // Hkv
+        g = torch.Generator(device="cuda").manual_seed(1)
+        kp = torch.randn(Hkv, N, D, device="cuda", generator=g).to(TDT[dt])
+        vp = torch.randn(Hkv, N, D, device="cuda", generator=g).to(TDT[dt])
+        sp = pkg.SharedPrefix(1)
+        sp.set(0, kp, vp)
+        qt = torch.from_numpy(q).cuda().to(TDT[dt])
+        out, lse = eng.attend(0, qt, prefix=sp, return_lse=True)
+        assert torch.equal(out, eng.attend(0, qt, prefix=sp))
+        rt, at = TOL[dt]
+        for b, oc in enumerate(seqs):
+            for h in range(Hkv):
+                K, V = kp[h].double().cpu().numpy(), vp[h].double().cpu().numpy()
+                if lens[b]:
+                    Kh, Vh, _ = oc.read_base_concat(0, h)
+                    K, V = np.concatenate([K, Kh]), np.concatenate([V, Vh])
+                S = q[b, h * grp:(h + 1) * grp].astype(np.float64) @ K.T / math.sqrt(D)
+                m = S.max(1, keepdims=True)
+                P = np.exp(S - m)
+                O = P @ V / P.sum(1, keepdims=True)
+                np.testing.assert_allclose(out[b, h * grp:(h + 1) * grp].double().cpu().numpy(), O, rtol=rt, atol=at)
+                np.testing.assert_allclose(lse[b, h * grp:(h + 1) * grp].cpu().numpy(), m[:, 0] + np.log(P.sum(1)),
+                                           rtol=1e-5, atol=LSE_TOL)
+
+
+def test_prefix_on_a_kv_head_shard(pkg):
+    """Two arenas with one kv head each give the rows of the unsharded call."""
+    with env(**PAPER_BEST_ENV):
+        D, Hq, Hkv, T = 64, 4, 2, 50
+        kw = dict(num_layers=1, head_dim=D, max_pages=8, base_bits=3, group_size=32, scale_quant="int8",
+                  packed_base=True, store_budget_mode="absolute", store_abs_k=1, store_abs_v=1,
+                  read_budget_mode="absolute", read_abs_k=1, read_abs_v=1, route_policy="joint", store_sketch=False)
+        g = torch.Generator(device="cuda").manual_seed(2)
+        K, V = (torch.randn(1, Hkv, T, D, device="cuda", generator=g).half() for _ in range(2))
+        kp, vp = (torch.randn(Hkv, 200, D, device="cuda", generator=g).half() for _ in range(2))
+        q = torch.randn(1, Hq, D, device="cuda", generator=g).half()
+
+        def run(h0, n, shard):
+            cfg = pkg.CacheConfig(num_heads=n * Hq // Hkv, num_kv_heads=n, **kw)
+            eng = pkg.DecodeEngine(pkg.CAREKVCache(cfg, torch.device("cuda"), batch=1), shard=shard)
+            eng.prefill_store(0, K, V)
+            sp = pkg.SharedPrefix(1)
+            sp.set(0, kp[h0:h0 + n], vp[h0:h0 + n])
+            return eng.attend(0, q, prefix=sp, return_lse=True)
+        whole, wl = run(0, 2, None)
+        for h in range(2):
+            part, pl = run(h, 1, (h, 2))
+            assert torch.equal(part[:, 2 * h:2 * h + 2], whole[:, 2 * h:2 * h + 2])
+            assert torch.equal(pl[:, 2 * h:2 * h + 2], wl[:, 2 * h:2 * h + 2])
+
+
+def rotated(x, positions, freq):
+    """x [..., T, H, D] float64, half layout."""
+    half = freq.numel()
+    ang = positions.double().unsqueeze(-1) * (freq.double() * (2 * math.pi / 2.0 ** 64))
+    c, s = torch.cos(ang).unsqueeze(-2), torch.sin(ang).unsqueeze(-2)
+    a, b = x[..., :half], x[..., half:2 * half]
+    return torch.cat((a * c - b * s, a * s + b * c, x[..., 2 * half:]), -1)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+def test_layer_step_with_4bit_weights_rotary_and_prefix(pkg, dt):
+    """Prefill and decode of a layer against the same mathematics in fp64 over the weights and the
+    cache contents that the layer holds."""
+    Hq, Hkv, D, dm, N, T, steps, B = 8, 2, 64, 96, 150, 21, 3, 3
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def rand(*s):
+        return torch.randn(*s, device="cuda", generator=g)
+    with env(CAREKV_PREFILL_MODE="fp", **PAPER_BEST_ENV):
+        cfg = pkg.CacheConfig(num_layers=1, num_heads=Hq, num_kv_heads=Hkv, head_dim=D, max_pages=4, base_bits=4,
+                              group_size=32, scale_quant="int8", packed_base=True, store_budget_mode="absolute",
+                              store_abs_k=1, store_abs_v=1, read_budget_mode="absolute", read_abs_k=0, read_abs_v=0,
+                              route_policy="joint", store_sketch=False)
+        ws = [(rand(o, i) / math.sqrt(i)).to(TDT[dt]) for o, i in ((Hq * D, dm), (Hkv * D, dm), (Hkv * D, dm),
+                                                                  (dm, Hq * D))]
+        layer = pkg.CAREKVLayer(cfg, 0, *ws, torch.device("cuda")).quantize_weights(32)
+        wq, wk, wv, wo = (layer._packed[n].dequantize().double() for n in ("W_Q", "W_K", "W_V", "W_O"))
+        layer.rotary = pkg.RotaryEmbedding(D, device="cuda")
+        sp = pkg.SharedPrefix(1)
+        sp.set(0, rand(Hkv, N, D).to(TDT[dt]), rand(Hkv, N, D).to(TDT[dt]))
+        kp, vp = (x.double().repeat_interleave(Hq // Hkv, 0) for x in sp.layer(0))
+        cache = pkg.CAREKVCache(cfg, torch.device("cuda"), batch=B)
+        hid = rand(B, T + steps, dm).to(TDT[dt])
+        pos = N + torch.arange(T + steps, device="cuda")
+        pre = layer.prefill_batch(cache, hid[:, :T], positions=pos[:T], prefix=sp)
+
+        def qkv(x, p):
+            x = x.double()
+            r = [(x @ w.T).view(*x.shape[:-1], -1, D) for w in (wq, wk, wv)]
+            return rotated(r[0], p, layer.rotary.freq), rotated(r[1], p, layer.rotary.freq), r[2]
+
+        def attend(q, k, v, own_mask=None):      # q [Hq, n, D]; k, v [Hkv, m, D] of the own tokens
+            k, v = (x.repeat_interleave(Hq // Hkv, 0) for x in (k, v))
+            s = q @ torch.cat((kp, k), 1).transpose(1, 2) / math.sqrt(D)
+            if own_mask is not None:
+                s[..., N:] = s[..., N:].masked_fill(own_mask, -math.inf)
+            return torch.softmax(s, -1) @ torch.cat((vp, v), 1)
+        rt, at = {"fp32": (1e-3, 2e-3), "fp16": (1e-2, 1e-2)}[dt]
+        causal = torch.triu(torch.ones(T, T, dtype=torch.bool, device="cuda"), 1)
+        for b in range(B):
+            q, k, v = (x.transpose(0, 1) for x in qkv(hid[b, :T], pos[:T]))
+            want = attend(q, k, v, causal).transpose(0, 1).reshape(T, -1) @ wo.T
+            np.testing.assert_allclose(pre[b].double().cpu(), want.cpu(), rtol=rt, atol=at)
+        for j in range(T, T + steps):
+            got = layer.decode_step_batch(cache, hid[:, j], positions=pos[j].expand(B), prefix=sp)
+            for b in range(B):
+                q, _, _ = qkv(hid[b, j:j + 1], pos[j:j + 1])
+                kc, ks, vc, vs = [], [], [], []
+                for h in range(Hkv):
+                    a = cache.read_base_concat(0, h, seq=b)
+                    kc.append(a[0].double() * a[1].double().repeat_interleave(32, 1))
+                    vc.append(a[2].double() * a[3].double().repeat_interleave(32, 1))
+                want = attend(q.transpose(0, 1), torch.stack(kc), torch.stack(vc)).reshape(1, -1) @ wo.T
+                np.testing.assert_allclose(got[b:b + 1].double().cpu(), want.cpu(), rtol=rt, atol=at)
+        cache.check_errors()
+
+
+def test_layer_refusals(pkg):
+    with env(CAREKV_PREFILL_MODE="carekv_stored", **PAPER_BEST_ENV):
+        cfg = pkg.CacheConfig(num_layers=1, num_heads=2, num_kv_heads=2, head_dim=64, max_pages=4, base_bits=3,
+                              group_size=32, scale_quant="int8", store_budget_mode="absolute", store_abs_k=1,
+                              store_abs_v=1, read_budget_mode="absolute", read_abs_k=1, read_abs_v=1)
+        W = torch.randn(128, 64, device="cuda")
+        layer = pkg.CAREKVLayer(cfg, 0, W, W, W, W.T.contiguous(), torch.device("cuda"))
+        cache = pkg.CAREKVCache(cfg, torch.device("cuda"), batch=1)
+        sp = pkg.SharedPrefix(1)
+        sp.set(0, torch.randn(2, 20, 64, device="cuda"), torch.randn(2, 20, 64, device="cuda"))
+        hid = torch.randn(1, 5, 64, device="cuda")
+        with pytest.raises(NotImplementedError, match="prefix"):
+            layer.prefill_batch(cache, hid, prefix=sp)
+        with pytest.raises(ValueError, match="rotary"):
+            layer.prefill_batch(cache, hid, positions=torch.arange(5, device="cuda"))
+        with pytest.raises(ValueError, match="has not been set"):
+            pkg.SharedPrefix(1).attend(0, torch.randn(1, 2, 64, device="cuda"))
