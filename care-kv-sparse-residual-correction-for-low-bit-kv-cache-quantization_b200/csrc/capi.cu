@@ -444,7 +444,7 @@ static int validate_w4_buffers(const carekv_w4_t* w) {
   CHECK(validate_w4(w));
   if (!w->codes || !w->scales) return CAREKV_ERR_INVALID_ARG;
   const uintptr_t m = reinterpret_cast<uintptr_t>(w->codes) | reinterpret_cast<uintptr_t>(w->scales);
-  return (m & 15) ? CAREKV_ERR_INVALID_ARG : CAREKV_OK;
+  return (m & 31) ? CAREKV_ERR_INVALID_ARG : CAREKV_OK;
 }
 
 int carekv_w4_layout(const carekv_w4_t* w, size_t sizes[2]) {

@@ -1,5 +1,6 @@
 // Host-side launch helpers.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace carekv {
@@ -27,6 +28,23 @@ cudaError_t allow_smem(K* kernel) {
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
   if (e == cudaSuccess && dev >= 0 && dev < 64) known[dev] = id;
   return e;
+}
+
+// cuTensorMapEncodeTiled, found through the runtime (no link against the
+// driver library); null where the driver has none.
+using TensorMapEncode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                     const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                     CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline TensorMapEncode tensor_map_encode() {
+  static const TensorMapEncode encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<TensorMapEncode>(f);
+  }();
+  return encode;
 }
 
 }  // namespace carekv

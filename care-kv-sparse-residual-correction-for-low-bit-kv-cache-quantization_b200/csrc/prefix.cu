@@ -165,20 +165,6 @@ struct TcLayout {
   static constexpr int kBytes = kBar + kBars * 8 + 16;
 };
 
-// A wait that gives up after about a second, or as soon as another wait of
-// the CTA has.
-__device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile int* dead) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity)) {
-    if (*dead || clock64() - t0 > (1ll << 31)) {
-      *dead = 1;
-      return false;
-    }
-  }
-  return true;
-}
-
 struct Segment {
   int kvh, rho0;      // first row of the tile within the kv head
   int b0, nb;         // token blocks that some row of the tile sees
@@ -225,21 +211,6 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-// two fp32 operations per instruction
-__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
-  float2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(*reinterpret_cast<uint64_t*>(&r))
-      : "l"(*reinterpret_cast<uint64_t*>(&x)), "l"(*reinterpret_cast<uint64_t*>(&y)), "l"(*reinterpret_cast<uint64_t*>(&z)));
-  return r;
-}
-__device__ __forceinline__ float2 add2(float2 x, float2 y) {
-  float2 r;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(*reinterpret_cast<uint64_t*>(&r))
-      : "l"(*reinterpret_cast<uint64_t*>(&x)), "l"(*reinterpret_cast<uint64_t*>(&y)));
-  return r;
 }
 // 2^y of two values on the FMA pipe, y >= -126 or clamped to it: y = n + f
 // with n the nearest integer (by adding 1.5 2^23), |f| <= 1/2, a degree-4
@@ -941,17 +912,7 @@ bool tc_shape(const carekv_prefix_t& p) {
 // [heads][tokens][D] with 64-channel x 128-token boxes.  A stride of an axis
 // of one element is never used; heads on one another (stride 0) are one head.
 bool tensor_map(CUtensorMap* map, const void* base, const carekv_prefix_t& p, const int64_t stride[2], int* head_step) {
-  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static Encode encode = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<Encode>(f);
-  }();
+  const TensorMapEncode encode = tensor_map_encode();
   if (!encode) return false;
   const int64_t row = static_cast<int64_t>(p.head_dim) * 2;
   const int64_t tok = p.tokens > 1 ? stride[1] * 2 : row;

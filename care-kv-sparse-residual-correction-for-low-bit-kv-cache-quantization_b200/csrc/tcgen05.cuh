@@ -136,6 +136,41 @@ __device__ __forceinline__ void tma_load_3d_pol(void* dst, const CUtensorMap* ma
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)), "l"(policy)
       : "memory");
 }
+// A wait that gives up after about a second, or as soon as another wait of
+// the CTA has (`dead`, in shared memory).
+__device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile int* dead) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*dead || clock64() - t0 > (1ll << 31)) {
+      *dead = 1;
+      return false;
+    }
+  }
+  return true;
+}
+// two fp32 operations per instruction
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*reinterpret_cast<uint64_t*>(&r))
+      : "l"(*reinterpret_cast<uint64_t*>(&x)), "l"(*reinterpret_cast<uint64_t*>(&y)), "l"(*reinterpret_cast<uint64_t*>(&z)));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(*reinterpret_cast<uint64_t*>(&r))
+      : "l"(*reinterpret_cast<uint64_t*>(&x)), "l"(*reinterpret_cast<uint64_t*>(&y)));
+  return r;
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_addr(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
+      : "memory");
+}
 __device__ __forceinline__ void named_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }

@@ -15,6 +15,7 @@
 #include "internal.h"
 #include "launch.h"
 #include "ptx.cuh"
+#include "tcgen05.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -32,7 +33,14 @@ namespace {
 // Nibble i of a word holds code + 8 of channel 2 i (i < 4) or 2 (i - 4) + 1,
 // so one mask picks the pair (2p, 2p + 1) into the two halves of a register.
 // Scales of a tile: [16 rows][ns], ns = 128 / group below 128, else 1.
-constexpr int kTileRows = 16, kTileK = 128, kTileBytes = 1024;
+// The 8 tiles (panels) of 128 rows at the same channels lie together, blocks
+// of 128 rows one after another: one 8 KB copy brings a block's tile (8
+// copies of 1 KB, a panel's tiles in a row, took 0.9 us a tile).
+constexpr int kTileRows = 16, kTileK = 128, kTileBytes = 1024, kBlockPanels = 8;
+
+__host__ __device__ inline int64_t tile_at(int64_t panel, int kt, int kt_n) {
+  return (panel / kBlockPanels * kt_n + kt) * kBlockPanels + panel % kBlockPanels;
+}
 
 __host__ __device__ inline int tile_scales(int group) { return group >= kTileK ? 1 : kTileK / group; }
 
@@ -43,8 +51,8 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* __restrict_
   if (w >= words) return;
   const int64_t tile = w >> 8;
   const int in = static_cast<int>(w & 255), hi = in >> 7, lane = (in >> 2) & 31, j = in & 3;
-  const int64_t panel = tile / kt_n;
-  const int kt = static_cast<int>(tile % kt_n);
+  const int64_t panel = tile / kBlockPanels / kt_n * kBlockPanels + tile % kBlockPanels;
+  const int kt = static_cast<int>(tile / kBlockPanels % kt_n);
   const int64_t n = panel * kTileRows + hi * 8 + (lane >> 2);
   const int k0 = kt * kTileK + 32 * j + 8 * (lane & 3);
   uint32_t v = 0x88888888u;   // code 0
@@ -76,9 +84,9 @@ __global__ void __launch_bounds__(256) w4_dequant_kernel(const uint32_t* __restr
   const int64_t tile = w >> 8;
   const int in = static_cast<int>(w & 255), hi = in >> 7, lane = (in >> 2) & 31, j = in & 3;
   const int row = hi * 8 + (lane >> 2);
-  const int64_t n = tile / kt_n * kTileRows + row;
+  const int64_t n = (tile / kBlockPanels / kt_n * kBlockPanels + tile % kBlockPanels) * kTileRows + row;
   const int kk = 32 * j + 8 * (lane & 3);
-  const int64_t k0 = tile % kt_n * kTileK + kk;
+  const int64_t k0 = tile / kBlockPanels % kt_n * kTileK + kk;
   if (n >= N || k0 >= K) return;
   const int ns = tile_scales(group);
   const float s = load_act(scales, tile * (kTileRows * ns) + row * ns + (ns > 1 ? kk / group : 0), dt);
@@ -258,7 +266,7 @@ __global__ void __launch_bounds__(WK * 32) w4_kernel(const typename Act<DT>::T* 
   const Scale* sp[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    const int64_t tile = static_cast<int64_t>(min(panel + r, panels - 1)) * kt_n + warp;
+    const int64_t tile = tile_at(min(panel + r, panels - 1), warp, kt_n);
     cp[r] = codes + tile * 64 + lane;
     sp[r] = reinterpret_cast<const Scale*>(scales) + tile * kTileRows + g;
   }
@@ -277,8 +285,8 @@ __global__ void __launch_bounds__(WK * 32) w4_kernel(const typename Act<DT>::T* 
       d[r].c1 = __ldg(cp[r] + 32);
       d[r].s0 = sp[r][0];
       d[r].s1 = sp[r][8];
-      cp[r] += WK * 64;
-      sp[r] += WK * kTileRows;
+      cp[r] += WK * kBlockPanels * 64;
+      sp[r] += WK * kBlockPanels * kTileRows;
     }
   };
   auto multiply = [&](const Tile<typename A::S, NS> (&d)[RT], int words) {
@@ -361,164 +369,241 @@ __global__ void __launch_bounds__(WK * 32) w4_kernel(const typename Act<DT>::T* 
   }
 }
 
-// More rows (up to 8 MT, 16-bit): the CTA's 8 warps take RT x 16 weight rows
-// each and share the activations; codes, scales and activations of the next
-// kWideStages - 1 tiles are on their way in shared memory.  The channels are
-// split over the CTAs of a cluster, which add their sums through distributed
-// shared memory in a fixed order.
-constexpr int kWideWarps = 8, kWideStages = 4;
-
-template <int NS, int MT, int RT>
-struct WideLayout {
-  static constexpr int kRows = kWideWarps * RT * kTileRows;
-  static constexpr int kX = 8 * MT * kTileK * 2;
-  static constexpr int kCodes = kWideWarps * RT * kTileBytes;
-  static constexpr int kScales = kRows * NS * 2;
-  static constexpr int kStage = kX + kCodes + kScales;
-  static constexpr int kSum = 8 * MT * (kRows + 1) * 4;   // [m][row], reuses the stages
-  static constexpr int kBytes = kSum > kWideStages * kStage ? kSum : kWideStages * kStage;
+// More rows (up to NT = 32 or 64, 16-bit) on tcgen05: a CTA takes 128
+// weight rows, the M side of the instruction, against the NT activation rows
+// of its N side.  A thread owns a weight row: it turns the row's 128 codes of
+// a tile into 16-bit numbers in 64 columns of its TMEM lane, from where the
+// instruction reads them as operand A, so the dequantized weight never passes
+// through shared memory (2 bytes per code written and read back there would
+// bound the kernel below HBM speed); the activations' tile is operand B, by
+// TMA.  Each scale group has a product sum of its own in TMEM, which the row's
+// thread multiplies by its scale and adds in fp32 registers: weights stay
+// exact.  Groups of four warps take the tiles in turn, each converting,
+// issuing its products (one warp issuing for all took 0.5 us a tile), waiting
+// for them and adding by itself; what hides the waits is the other groups' work, so there are as many as the registers allow (the NT
+// sums of a row are held by each).  Codes and scales come through shared
+// memory too, by bulk copies several tiles ahead: with the two tiles a thread
+// could hold in registers the loads in flight bounded the kernel (5120 rows
+// of 13824 channels, 64 activation rows: 35.5 us instead of 28.6).  The channels are split over the CTAs of a
+// cluster, which add their sums through distributed shared memory in a fixed
+// order.
+template <int NS, int NT>
+struct TcLayout {
+  static constexpr int kStages = NT == 64 ? 6 : 8;
+  static constexpr int kGroups = NT == 32 ? 3 : 2;                  // of four warps, 128 or 168 registers a thread
+  static constexpr int kSums = NT == 64 ? 2 : 1;                    // 64-column buffers of sums per group
+  static constexpr int kThreads = kGroups * 128 + 32;
+  static constexpr int kX = NT * kTileK * 2;                        // one tile of activations
+  static constexpr int kCodes = kX, kScales = kCodes + kBlockPanels * kTileBytes;   // of the tile's 8 panels
+  static constexpr int kBytesIn = kScales + 128 * NS * 2;
+  static constexpr int kStage = (kBytesIn + 1023) / 1024 * 1024;
+  static constexpr int kPart = kStages * kStage;                    // float [kGroups - 1][NT][128]
+  static constexpr int kBar = kPart + (kGroups - 1) * NT * 128 * 4;
+  static constexpr int kBars = 2 * kStages + kGroups * kSums + 1;
+  static constexpr int kBytes = kBar + kBars * 8 + 16;
+  static_assert(kGroups * (64 + 64 * kSums) <= 512, "TMEM columns");
 };
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(in ? 16 : 0)
-               : "memory");
-}
-
-template <int DT, int NS, int MT, int RT>
-__global__ void __launch_bounds__(kWideWarps * 32) w4_wide_kernel(const typename Act<DT>::T* __restrict__ x, int64_t ldx,
-                                                                  int M, const uint4* __restrict__ codes,
-                                                                  const typename Act<DT>::S* __restrict__ scales, int N,
-                                                                  int K, int kt_n, int panels, const Keys keys,
-                                                                  typename Act<DT>::T* __restrict__ out) {
+template <int DT, int NS, int NT>
+__global__ void __launch_bounds__(TcLayout<NS, NT>::kThreads, 1)
+    w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, int M, const uint4* __restrict__ codes,
+                 const typename Act<DT>::S* __restrict__ scales, int N, int kt_n, const Keys keys, typename Act<DT>::T* __restrict__ out) {
   using A = Act<DT>;
-  using Ly = WideLayout<NS, MT, RT>;
+  using Ly = TcLayout<NS, NT>;
   using Scale = ScaleVec<typename A::S, NS>;
-  constexpr int kPer = 4 / NS, kThreads = kWideWarps * 32;
-  extern __shared__ __align__(16) unsigned char sm[];
+  constexpr int W = Ly::kGroups, kLoad = 4 * W, kCols = 64 + 64 * Ly::kSums;
+  constexpr int kSteps = kTileK / 16 / NS;   // instructions per scale group
+  // scale groups handed over at once: as many as 64 columns of sums hold
+  constexpr int kBatch = NS < 64 / NT ? NS : 64 / NT, kBatches = NS / kBatch;
+  extern __shared__ __align__(1024) unsigned char sm[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Ly::kBar);
+  // a stage has come / been read; per group of warps and buffer: sums ready
+  uint64_t *x_full = bars, *x_empty = bars + Ly::kStages, *d_full = bars + 2 * Ly::kStages,
+           *done = d_full + W * Ly::kSums;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Ly::kBars);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
   cg::cluster_group cluster = cg::this_cluster();
   const int splits = cluster.num_blocks(), split = cluster.block_rank();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int row0 = (blockIdx.x / splits) * Ly::kRows;
-  const int m0 = blockIdx.y * 8 * MT;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row0 = (blockIdx.x / splits) * 128, m0 = blockIdx.y * NT;
   const int kt0 = static_cast<int>(static_cast<int64_t>(kt_n) * split / splits);
-  const int kt1 = static_cast<int>(static_cast<int64_t>(kt_n) * (split + 1) / splits);
-
-  // this thread's 16-byte pieces of a stage; weight rows past the last panel
-  // repeat it (their sums are not stored), activation rows past the last and
-  // channels past K are zero.  Chunk c of activation row m lies at
-  // c ^ 4 (m & 1), so that the 2 rows x 4 chunks a quarter warp reads fall on
-  // different banks.
-  constexpr int kCodePieces = kWideWarps * RT * 64 / kThreads, kXPieces = 8 * MT * 16 / kThreads;
-  const uint4* code_src[kCodePieces];
-#pragma unroll
-  for (int i = 0; i < kCodePieces; ++i) {
-    const int at = threadIdx.x + i * kThreads;
-    const int64_t panel = min(row0 / kTileRows + (at >> 6), panels - 1);
-    code_src[i] = codes + (panel * kt_n + kt0) * 64 + (at & 63);
-  }
-  constexpr int kScalePieces = Ly::kScales / 16;   // at most 512 bytes x RT x ...: one or two per thread
-  constexpr int kPanelPieces = kTileRows * NS * 2 / 16;
-  auto stage = [&](int kt) {
-    if (kt < kt1) {
-      unsigned char* d = sm + (kt % kWideStages) * Ly::kStage;
-#pragma unroll
-      for (int i = 0; i < kXPieces; ++i) {
-        const int at = threadIdx.x + i * kThreads, m = at >> 4, c = at & 15, k = kt * kTileK + 8 * c;
-        const bool in = m0 + m < M && k < K;
-        cp_async16(d + m * 256 + ((c ^ ((m & 1) << 2)) << 4), in ? x + (m0 + m) * ldx + k : x, in);
-      }
-      d += Ly::kX;
-#pragma unroll
-      for (int i = 0; i < kCodePieces; ++i) {
-        cp_async16(d + (threadIdx.x + i * kThreads) * 16, code_src[i], true);
-        code_src[i] += 64;
-      }
-      d += Ly::kCodes;
-      for (int i = threadIdx.x; i < kScalePieces; i += kThreads) {
-        const int64_t panel = min(row0 / kTileRows + i / kPanelPieces, panels - 1);
-        cp_async16(d + i * 16, scales + (panel * kt_n + kt) * (kTileRows * NS) + i % kPanelPieces * 8, true);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+  const int tiles = static_cast<int>(static_cast<int64_t>(kt_n) * (split + 1) / splits) - kt0;
+  float* part = reinterpret_cast<float*>(sm + Ly::kPart);
+  bool ok = true;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    ok = ok && __all_sync(0xffffffffu, wait_or(bar, parity, dead));
   };
-#pragma unroll
-  for (int i = 0; i < kWideStages - 1; ++i) stage(kt0 + i);
-  float acc[RT][MT][4] = {};
-  for (int kt = kt0; kt < kt1; ++kt) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kWideStages - 2) : "memory");
-    __syncthreads();   // tile kt has landed for all; the stage of tile kt - 1 is free
-    stage(kt + kWideStages - 1);
-    const unsigned char* d = sm + (kt % kWideStages) * Ly::kStage;
-    Tile<typename A::S, NS> cur[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const uint4* c = reinterpret_cast<const uint4*>(d + Ly::kX + (warp * RT + r) * kTileBytes);
-      cur[r].c0 = c[lane];
-      cur[r].c1 = c[lane + 32];
-      const Scale* s = reinterpret_cast<const Scale*>(d + Ly::kX + Ly::kCodes) + (warp * RT + r) * kTileRows;
-      cur[r].s0 = s[g];
-      cur[r].s1 = s[g + 8];
+  if (warp == kLoad) tmem_alloc(tmem_slot, 512);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Ly::kStages; ++i) {
+      mbar_init(x_full + i, 1);
+      mbar_init(x_empty + i, 1);
     }
-    const unsigned char* xs = d + g * 256;
-    float sum[RT][MT][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t a[RT][4], b[RT][4];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        codes8<A::kF16>(word(cur[r].c0, j), keys, a[r]);
-        codes8<A::kF16>(word(cur[r].c1, j), keys, b[r]);
+    for (int i = 0; i < W * Ly::kSums; ++i) mbar_init(d_full + i, 1);
+    mbar_init(done, W);
+    *dead = 0;
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;   // group w: A at kCols w, sums at kCols w + 64 + 64 buffer
+  if (warp == kLoad) {
+    int i = 0;
+    const int64_t tile0 = tile_at(row0 / kTileRows, kt0, kt_n);
+    for (; i < tiles && ok; ++i) {
+      const int s = i % Ly::kStages;
+      wait(x_empty + s, ((i / Ly::kStages) & 1) ^ 1);
+      if (!ok) break;
+      unsigned char* st = sm + s * Ly::kStage;
+      if (lane == 0) {
+        mbar_expect_tx(x_full + s, Ly::kBytesIn);
+        tma_load_2d(st, &xmap, (kt0 + i) * kTileK, m0, x_full + s);
+        tma_load_2d(st + NT * 128, &xmap, (kt0 + i) * kTileK + 64, m0, x_full + s);
+        const int64_t tile = tile0 + static_cast<int64_t>(i) * kBlockPanels;
+        bulk_g2s(st + Ly::kCodes, codes + tile * 64, kBlockPanels * kTileBytes, x_full + s);
+        bulk_g2s(st + Ly::kScales, scales + tile * (kTileRows * NS), 128 * NS * 2, x_full + s);
       }
-uint32_t xb[MT][1][4];
+    }
+    // a copy in flight must land before the CTA ends (all have when ok)
+    if (!ok)
+      for (int j = max(0, i - Ly::kStages); j < i; ++j) mbar_wait(x_full + j % Ly::kStages, (j / Ly::kStages) & 1);
+  } else {
+    const int w = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t base = tmem + kCols * w + (static_cast<uint32_t>(warp & 3) << 21);
+    // the group's first warp issues its products
+    constexpr uint32_t kId = mma_idesc(128, NT, !A::kF16, false);
+    const bool issuer = (warp & 3) == 0;
+    const uint32_t lead = elect_one();
+    const uint64_t xd = smem_desc(smem_addr(sm), 16, 1024);
+    auto products = [&](int s, int batch, int c) {
 #pragma unroll
-      for (int n = 0; n < MT; ++n) {
-        const uint4 v = *reinterpret_cast<const uint4*>(xs + n * (8 * 256) + (((4 * j + t) ^ ((g & 1) << 2)) << 4));
-        xb[n][0][0] = v.x, xb[n][0][1] = v.y, xb[n][0][2] = v.z, xb[n][0][3] = v.w;
+      for (int g = 0; g < kBatch; ++g)
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          const int step = (batch * kBatch + g) * kSteps + k;
+          mma_ts(tmem + kCols * w + 64 + 64 * (c % Ly::kSums) + g * NT, tmem + kCols * w + 8 * step,
+                 xd + s * (Ly::kStage / 16) + (step / 4) * (NT * 128 / 16) + (step % 4) * 2, kId, k > 0, lead);
+        }
+      mma_commit(d_full + w * Ly::kSums + c % Ly::kSums, lead);
+    };
+    float2 acc[NT / 2];
+#pragma unroll
+    for (int i = 0; i < NT / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+    // one tile: its products follow its codes, so A is free when the last
+    // sums of the tile before it have come
+    for (int i = w, n = 0; i < tiles; i += W, ++n) {
+      const int s = i % Ly::kStages;
+      wait(x_full + s, (i / Ly::kStages) & 1);
+      Scale sc;
+      if (ok) {
+        // the row's 64 bytes: word j of channels 32 j + 8 t .. in c[t]
+        const unsigned char* st = sm + s * Ly::kStage;
+        const uint4* cp = reinterpret_cast<const uint4*>(st + Ly::kCodes) + row * 4;
+        const uint4 c[4] = {cp[0], cp[1], cp[2], cp[3]};
+        sc = reinterpret_cast<const Scale*>(st + Ly::kScales)[row];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t v[16];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            uint32_t q[4];
+            codes8<A::kF16>(word(c[t], j), keys, q);
+#pragma unroll
+            for (int p = 0; p < 4; ++p) v[4 * t + p] = q[p];
+          }
+          tmem_st16(base + 16 * j, v);
+        }
+        tmem_wait_st();
       }
-      // products that share a sum are MT RT apart
+      tc_fence_before();
+      named_sync(2 + w, 128);   // the whole tile is converted, the sums before it are taken
+      tc_fence_after();
+      constexpr int kAhead = kBatches < Ly::kSums ? kBatches : Ly::kSums;
+      if (ok && issuer) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+        for (int b = 0; b < kAhead; ++b) products(s, b, n * kBatches + b);
+        if (kAhead == kBatches) mma_commit(x_empty + s, lead);
+      }
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+      for (int b = 0; b < kBatches; ++b) {
+        const int c = n * kBatches + b;
+        wait(d_full + w * Ly::kSums + c % Ly::kSums, (c / Ly::kSums) & 1);
+        tc_fence_after();
+        if (ok) {
+          constexpr int kLd = 32;
 #pragma unroll
-          for (int n = 0; n < MT; ++n) mma_half<A>(sum[r][n], a[r], b[r], xb[n], h, j % kPer == 0 && h == 0);
-      if (j % kPer == kPer - 1) {
+          for (int h = 0; h < kBatch * NT; h += kLd) {
+            const float f = A::scale(sc.v[b * kBatch + h / NT]);
+            uint32_t x[kLd];
+            tmem_ld32(base + 64 + 64 * (c % Ly::kSums) + h, x);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const float s0 = A::scale(cur[r].s0.v[j / kPer]), s1 = A::scale(cur[r].s1.v[j / kPer]);
-#pragma unroll
-          for (int n = 0; n < MT; ++n) add_scaled(acc[r][n], sum[r][n], s0, s1);
+            for (int i = 0; i < kLd / 2; ++i) {
+              float2& y = acc[(h % NT) / 2 + i];
+              y = fma2(make_float2(f, f), make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), y);
+            }
+          }
+        }
+        if (b + kAhead < kBatches) {   // the buffer's next sums, when all four warps have taken these
+          tc_fence_before();
+          named_sync(2 + w, 128);
+          tc_fence_after();
+          if (ok && issuer) {
+            products(s, b + kAhead, c + kAhead);
+            if (b + kAhead + 1 == kBatches) mma_commit(x_empty + s, lead);
+          }
         }
       }
     }
+    if (issuer) {   // nothing of ours may still run or arrive when the CTA ends
+      mma_commit(done, lead);
+      mbar_wait(done, 0);
+    }
+    __syncwarp();
+    if (!ok) {   // a wait ran out: the rows say so
+#pragma unroll
+      for (int i = 0; i < NT / 2; ++i) acc[i] = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
+    }
+    if (w > 0) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) part[((w - 1) * NT + i) * 128 + row] = (i & 1) ? acc[i / 2].y : acc[i / 2].x;
+    }
+    named_sync(1, W * 128);
+    if (w == 0) {
+      const int n0 = row0 + row;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        float v = (i & 1) ? acc[i / 2].y : acc[i / 2].x;
+#pragma unroll
+        for (int g = 0; g < W - 1; ++g) v += part[(g * NT + i) * 128 + row];
+        if (splits > 1) part[i * 128 + row] = v;
+        else if (m0 + i < M && n0 < N) out[static_cast<int64_t>(m0 + i) * N + n0] = A::out(v);
+      }
+    }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  float* part = reinterpret_cast<float*>(sm);
-  constexpr int kLd = Ly::kRows + 1;
+  tc_fence_before();
+  if (splits > 1) {
+    cluster.sync();
+    // every CTA finishes its share of the activation rows
+    if (warp < 4 * W) {
+      const int mn = min(NT, M - m0), r = threadIdx.x & 127;
+      for (int m = split + splits * (threadIdx.x >> 7); m < mn; m += W * splits) {
+        float v = 0.f, p[8];   // all reads on their way before the first sum
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+        for (int s = 0; s < 8; ++s) p[s] = s < splits ? cluster.map_shared_rank(part, s)[m * 128 + r] : 0.f;
 #pragma unroll
-    for (int n = 0; n < MT; ++n) {
-      float* p = part + (8 * n + 2 * t) * kLd + (warp * RT + r) * kTileRows + g;
-      p[0] = acc[r][n][0];
-      p[kLd] = acc[r][n][1];
-      p[8] = acc[r][n][2];
-      p[kLd + 8] = acc[r][n][3];
+        for (int s = 0; s < 8; ++s) v += p[s];
+        if (row0 + r < N) out[static_cast<int64_t>(m0 + m) * N + row0 + r] = A::out(v);
+      }
     }
-  cluster.sync();
-  // every CTA finishes its share of the activation rows
-  const int mn = min(8 * MT, M - m0);
-  for (int m = split; m < mn; m += splits)
-    for (int r = threadIdx.x; r < Ly::kRows && row0 + r < N; r += kThreads) {
-      float v = 0.f, p[8];   // all reads on their way before the first sum
-#pragma unroll
-      for (int s = 0; s < 8; ++s) p[s] = s < splits ? cluster.map_shared_rank(part, s)[m * kLd + r] : 0.f;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) v += p[s];
-      out[static_cast<int64_t>(m0 + m) * N + row0 + r] = A::out(v);
-    }
-  cluster.sync();   // no CTA leaves while another reads its sums
+    cluster.sync();   // no CTA leaves while another reads its sums
+  } else {
+    __syncthreads();
+  }
+  if (warp == kLoad) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
 }
 
 template <int DT, int NS, int MT, int RT, int WK>
@@ -532,21 +617,59 @@ cudaError_t launch_few(const carekv_w4_t& w, const void* x, int64_t ldx, int M, 
                                                           panels, kKeys<A::kF16>, static_cast<typename A::T*>(out));
   return cudaGetLastError();
 }
-template <int DT, int NS, int MT, int RT>
-cudaError_t launch_wide(const carekv_w4_t& w, const void* x, int64_t ldx, int M, void* out, cudaStream_t st) {
+// Clusters of 1 .. 8 CTAs of `kernel` that the device holds at once.
+template <typename K>
+int max_clusters(K* kernel, int size, int threads, int smem) {
+  static thread_local const void* known[9] = {};
+  static thread_local int count[9] = {};
+  if (known[size] == reinterpret_cast<const void*>(kernel)) return count[size];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {static_cast<unsigned>(size), 1, 1};
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  known[size] = reinterpret_cast<const void*>(kernel);
+  count[size] = n;
+  return n;
+}
+
+template <int DT, int NS, int NT>
+cudaError_t launch_tc(const carekv_w4_t& w, const void* x, int64_t ldx, int M, void* out, cudaStream_t st) {
   using A = Act<DT>;
-  using Ly = WideLayout<NS, MT, RT>;
-  const int kt_n = (w.k + kTileK - 1) / kTileK, panels = (w.n + kTileRows - 1) / kTileRows;
-  const int blocks = (w.n + Ly::kRows - 1) / Ly::kRows, cols = (M + 8 * MT - 1) / (8 * MT);
-  // CTAs of a cluster: as many as fill the GPU, at least 4 tiles of channels each
-  constexpr int kPerSm = MT == 2 ? 2 : 1;
-  const int splits = std::max(1, std::min({8, kPerSm * 148 / (blocks * cols), kt_n / 4}));
-  auto kernel = w4_wide_kernel<DT, NS, MT, RT>;
+  using Ly = TcLayout<NS, NT>;
+  const int kt_n = (w.k + kTileK - 1) / kTileK;
+  const int blocks = (w.n + 127) / 128, cols = (M + NT - 1) / NT;
+  const TensorMapEncode encode = tensor_map_encode();
+  if (!encode) return cudaErrorNotSupported;
+  // activations [M][k] in boxes of NT rows x 64 channels; rows and channels
+  // past the end read as zero
+  CUtensorMap map;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(w.k), static_cast<cuuint64_t>(M)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ldx) * 2};
+  const cuuint32_t box[2] = {64, NT}, step[2] = {1, 1};
+  if (encode(&map, DT == CAREKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+             const_cast<void*>(x), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return cudaErrorInvalidValue;
+  auto kernel = w4_tc_kernel<DT, NS, NT>;
   const cudaError_t e = allow_smem<Ly::kBytes>(kernel);
   if (e != cudaSuccess) return e;
+  // CTAs of a cluster: the most that still run all at once, at least 4 tiles each
+  int splits = 1;
+  for (int s = 2; s <= 8 && blocks * cols * s <= sm_count() && kt_n >= 4 * s; ++s)
+    if (blocks * cols <= max_clusters(kernel, s, Ly::kThreads, Ly::kBytes)) splits = s;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks * splits, cols);
-  cfg.blockDim = dim3(kWideWarps * 32);
+  cfg.blockDim = dim3(Ly::kThreads);
   cfg.dynamicSmemBytes = Ly::kBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -554,15 +677,22 @@ cudaError_t launch_wide(const carekv_w4_t& w, const void* x, int64_t ldx, int M,
   attr.val.clusterDim = {static_cast<unsigned>(splits), 1, 1};
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<const typename A::T*>(x), ldx, M,
-                            static_cast<const uint4*>(w.codes), static_cast<const typename A::S*>(w.scales), w.n, w.k,
-                            kt_n, panels, kKeys<A::kF16>, static_cast<typename A::T*>(out));
+  return cudaLaunchKernelEx(&cfg, kernel, map, M, static_cast<const uint4*>(w.codes),
+                            static_cast<const typename A::S*>(w.scales), w.n, kt_n, kKeys<A::kF16>,
+                            static_cast<typename A::T*>(out));
 }
-// Which form: up to 8 rows the few-row kernel, with as many warps per 16
-// weight rows as the number of such panels leaves room for (1 row, us per
-// call with 4 / 8 / 16 warps: 864 panels of 5120 channels 11.1 / 11.9 / 13.3,
-// 320 panels of 13824 18.8 / 13.0 / 15.1, 256 panels of 4096 5.5 / 4.4 / 4.2);
-// above that the wide kernel.
+// Which form.  Up to 16 rows (any number in fp32) the few-row kernel, with as
+// many warps per 16 weight rows as the number of such panels leaves room for.
+// Measured with 4 / 8 / 16 warps, us per call:
+//   1 row:   864 panels of 5120 channels 11.1 / 11.9 / 13.3, 320 of 13824
+//            18.8 / 13.0 / 15.1, 256 of 4096 5.5 / 4.4 / 4.2
+//   16 rows: 864 panels of 5120 (two panels a CTA with 4 warps) 14.9 / 17.5 /
+//            24.7, 320 of 13824 27.5 / 19.4 / 26.9, 64 of 4096 6.9 / 5.4 / 3.9
+// Beyond 16 rows that kernel reads the weight again for every 16, and the
+// tcgen05 kernel takes over where the weight is large: 32 rows x 14336 x 4096
+// 28.5 against 21.3 us, but 32 x 4096 x 4096 8.5 against 9.6; 64 x 5120 x
+// 13824 56 against 28.6, 40 x 5632 x 2048 11.3 against 11.2, 48 x 700 x 512
+// 2.7 against 9.5.
 template <int DT, int NS>
 cudaError_t launch_ns(const carekv_w4_t& w, const void* x, int64_t ldx, int M, void* out, cudaStream_t st) {
   const int panels = (w.n + kTileRows - 1) / kTileRows;
@@ -572,8 +702,12 @@ cudaError_t launch_ns(const carekv_w4_t& w, const void* x, int64_t ldx, int M, v
     return launch_few<DT, NS, 1, 1, 16>(w, x, ldx, M, out, st);
   }
   if constexpr (DT != CAREKV_F32) {
-    if (M <= 16) return launch_wide<DT, NS, 2, 2>(w, x, ldx, M, out, st);
-    return launch_wide<DT, NS, 4, 2>(w, x, ldx, M, out, st);
+    const int64_t codes = static_cast<int64_t>(w.n) * w.k;
+    if (M > 32 && codes >= (8 << 20)) return launch_tc<DT, NS, 64>(w, x, ldx, M, out, st);
+    if (M > 16 && M <= 32 && codes >= (32 << 20)) return launch_tc<DT, NS, 32>(w, x, ldx, M, out, st);
+    if (panels >= (M > 16 ? 148 : 4 * 148)) return launch_few<DT, NS, 2, 2, 4>(w, x, ldx, M, out, st);
+    if (panels >= 148) return launch_few<DT, NS, 2, 1, 8>(w, x, ldx, M, out, st);
+    return launch_few<DT, NS, 2, 1, 16>(w, x, ldx, M, out, st);
   }
   return cudaErrorInvalidValue;
 }
@@ -587,7 +721,7 @@ cudaError_t launch_dt(const carekv_w4_t& w, const void* x, int64_t ldx, int M, v
 }
 
 int64_t tiles(int n, int k) {
-  return static_cast<int64_t>((n + kTileRows - 1) / kTileRows) * ((k + kTileK - 1) / kTileK);
+  return static_cast<int64_t>((n + 127) / 128) * kBlockPanels * ((k + kTileK - 1) / kTileK);
 }
 
 }  // namespace

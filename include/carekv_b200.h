@@ -459,7 +459,7 @@ int carekv_rotary(const carekv_rotary_t *args, void *stream);
 /* 4-bit weights [n][k] with one scale per group of group_size channels (32,
  * 64 or a multiple of 128 dividing k), held in the layout of the product
  * kernels.  codes and scales are device buffers of the sizes that
- * carekv_w4_layout gives, 16-byte aligned, filled once by carekv_w4_pack
+ * carekv_w4_layout gives, 32-byte aligned, filled once by carekv_w4_pack
  * from packed rows [n][k / 2] (carekv_pack_codes, bits 4) and scales
  * [n][k / group_size] in `dtype`.  No counterpart in the reference, whose
  * projections stay in the model's dtype. */
