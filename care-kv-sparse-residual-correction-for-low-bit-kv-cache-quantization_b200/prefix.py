@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._tensors import dtype_code, need_cuda, need_like, new_rows, on_device, rows_of, stream
+from ._tensors import dtype_code, launch, need_cuda, need_like, new_rows, rows_of
 
 
 def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = None,
@@ -51,7 +51,8 @@ def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = N
         raise ValueError(f"prefix_attention: {hq} query heads over {hkv} kv heads")
     q, k, v = rows_of(q), rows_of(k), rows_of(v)
     if lengths is not None:
-        if lengths.device != q.device or lengths.dtype is not torch.int32 or tuple(lengths.shape) != (n,):
+        if lengths.get_device() != q.get_device() or lengths.dtype is not torch.int32 or lengths.dim() != 1 \
+                or lengths.shape[0] != n:
             raise ValueError(f"prefix_attention lengths: expected int32 [{n}] on {q.device}")
         lengths = lengths.contiguous()
     tail_o = tail_lse = None
@@ -69,26 +70,27 @@ def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = N
         if out.shape != q.shape or not out.is_contiguous():
             raise ValueError(f"prefix_attention out: expected a contiguous tensor of shape {tuple(q.shape)}")
     lse = q.new_empty((n, hq), dtype=torch.float32) if return_lse else None
-    prefix = _lib.PREFIX_PACK(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), hkv,
-                              tokens, d, dt)
-    with on_device(q):
-        need = _workspace_bytes(n, hq, hkv, tokens, d, dt, q.get_device())
-        ws = q.new_empty(need, dtype=torch.uint8)
-        status = _lib.lib().carekv_prefix_attention(
-            prefix, q.data_ptr(), q.stride(0), q.stride(1), n, hq, 1.0 / math.sqrt(d) if scale is None else scale,
-            None if lengths is None else lengths.data_ptr(), None if tail_o is None else tail_o.data_ptr(),
-            None if tail_lse is None else tail_lse.data_ptr(), out.data_ptr(),
-            None if lse is None else lse.data_ptr(), ws.data_ptr(), need, stream(q))
-    if status:
-        _lib.check(status, "carekv_prefix_attention")
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
+    prefix = _lib.PREFIX_PACK(k.data_ptr(), v.data_ptr(), k0, k1, v0, v1, hkv, tokens, d, dt)
+    index = q.get_device()
+    need = _workspace_bytes(n, hq, hkv, tokens, d, dt, index)
+    ws = torch.empty(need, dtype=torch.uint8, device=index) if need else None
+    row, head, _ = q.stride()
+    launch(_lib.lib().carekv_prefix_attention, q, "carekv_prefix_attention", prefix, q.data_ptr(), row, head, n, hq,
+           1.0 / math.sqrt(d) if scale is None else scale, None if lengths is None else lengths.data_ptr(),
+           None if tail_o is None else tail_o.data_ptr(), None if tail_lse is None else tail_lse.data_ptr(),
+           out.data_ptr(), None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(n, hq, hkv, tokens, d, dt, _device) -> int:
+def _workspace_bytes(n, hq, hkv, tokens, d, dt, device) -> int:
+    """Workspace of a shape on a device (its number of SMs enters)."""
     need = ctypes.c_size_t(0)
-    _lib.check(_lib.lib().carekv_prefix_workspace_bytes(_lib.PREFIX_PACK(0, 0, 0, 0, 0, 0, hkv, tokens, d, dt), n, hq,
-                                                        ctypes.byref(need)), "carekv_prefix_workspace_bytes")
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().carekv_prefix_workspace_bytes(_lib.PREFIX_PACK(0, 0, 0, 0, 0, 0, hkv, tokens, d, dt), n,
+                                                            hq, ctypes.byref(need)), "carekv_prefix_workspace_bytes")
     return need.value
 
 

@@ -17,7 +17,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._tensors import dtype_code, need_cuda, need_like, new_rows, on_device, rows_of, stream
+from ._tensors import dtype_code, launch, need_cuda, need_like, new_rows, rows_of
 
 LAYOUTS = ("half", "interleaved")
 
@@ -146,9 +146,11 @@ def _turn(q, k, positions, freq, layout, attention_factor, inverse, out):
     batch, tokens = (shape[0], shape[1]) if nd == 4 else (1, shape[0])
     if k is not None:
         need_like(k, q, "apply_rotary k")
-        if k.dim() != nd or k.shape[:-2] != shape[:-2] or k.shape[-1] != D:
-            raise ValueError(f"apply_rotary k: {tuple(k.shape)} does not match q {tuple(shape)}")
-    if positions.device != q.device or freq.device != q.device:
+        ks = k.shape
+        if len(ks) != nd or ks[0] != shape[0] or ks[-1] != D or (nd == 4 and ks[1] != tokens):
+            raise ValueError(f"apply_rotary k: {tuple(ks)} does not match q {tuple(shape)}")
+    index = q.get_device()
+    if positions.get_device() != index or freq.get_device() != index:
         raise RuntimeError(f"apply_rotary: positions and freq belong on {q.device}")
     if positions.dtype is torch.int64:
         position_bytes = 8
@@ -179,10 +181,7 @@ def _turn(q, k, positions, freq, layout, attention_factor, inverse, out):
     args = _lib.ROTARY_PACK(*_rows(q, yq), *(_NO_ROWS if k is None else _rows(k, yk)), freq.data_ptr(),
                             positions.data_ptr(), sb, stok, position_bytes, batch, tokens, D, rd,
                             layout == "interleaved", bool(inverse), attention_factor, dt)
-    with on_device(q):
-        status = _lib.lib().carekv_rotary(args, stream(q))
-    if status:
-        _lib.check(status, "carekv_rotary")
+    launch(_lib.lib().carekv_rotary, q, "carekv_rotary", args)
     return yq, yk
 
 

@@ -14,7 +14,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._tensors import dtype_code, need_cuda, need_like, on_device, stream
+from ._tensors import dtype_code, launch, need_cuda, need_like
 from .quantizer import QuantConfig, pack_codes_2d, quantize
 
 # rows up to which matmul multiplies from the codes (PackedWeight.matmul)
@@ -53,9 +53,8 @@ class PackedWeight:
         self.scales = torch.empty(sizes[1], dtype=torch.uint8, device=packed.device)
         self.c.codes, self.c.scales = self.codes.data_ptr(), self.scales.data_ptr()
         self._ref, self._index = ctypes.byref(self.c), packed.get_device()
-        with on_device(packed):
-            _lib.check(lib.carekv_w4_pack(ctypes.byref(self.c), packed.data_ptr(), scale.data_ptr(), stream(packed)),
-                       "carekv_w4_pack")
+        launch(lib.carekv_w4_pack, packed, "carekv_w4_pack", ctypes.byref(self.c), packed.data_ptr(),
+               scale.data_ptr())
 
     @classmethod
     def from_dense(cls, weight: Tensor, group_size: int = 32) -> "PackedWeight":
@@ -79,8 +78,11 @@ class PackedWeight:
             raise ValueError(f"matvec x: expected [..., {k}], got {tuple(shape)}")
         # rows the kernel can read in place: unit channel stride, every row
         # on a 16-byte boundary
-        flat = x
-        if len(shape) != 2 or x.stride(1) != 1 or x.stride(0) < k or x.stride(0) % 8:
+        flat, plain = x, len(shape) == 2
+        if plain:
+            step, one = x.stride()
+            plain = one == 1 and step >= k and step % 8 == 0
+        if not plain:
             flat = x.reshape(-1, k).contiguous()
         if flat.data_ptr() % 16:
             flat = flat.clone(memory_format=torch.contiguous_format)
@@ -91,19 +93,14 @@ class PackedWeight:
             need_like(out, x, "matvec out")
             if tuple(out.shape) != (*shape[:-1], n) or not out.is_contiguous():
                 raise ValueError(f"matvec out: expected a contiguous tensor of shape {(*shape[:-1], n)}")
-        with on_device(x):
-            status = _lib.lib().carekv_w4_matvec(self._ref, flat.data_ptr(), max(flat.stride(0), k), rows,
-                                                 out.data_ptr(), stream(x))
-        if status:
-            _lib.check(status, "carekv_w4_matvec")
+        launch(_lib.lib().carekv_w4_matvec, x, "carekv_w4_matvec", self._ref, flat.data_ptr(),
+               max(flat.stride(0), k), rows, out.data_ptr())
         return out
 
     def dequantize(self) -> Tensor:
         """The dense weight [N, K], codes * scale rounded to the scales' dtype."""
         out = torch.empty(self.shape, dtype=self.dtype, device=self.device)
-        with on_device(out):
-            _lib.check(_lib.lib().carekv_w4_dequantize(ctypes.byref(self.c), out.data_ptr(), stream(out)),
-                       "carekv_w4_dequantize")
+        launch(_lib.lib().carekv_w4_dequantize, out, "carekv_w4_dequantize", self._ref, out.data_ptr())
         return out
 
     def matmul(self, x: Tensor) -> Tensor:
