@@ -37,6 +37,15 @@ def new_rows(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t) if t.is_contiguous() else t.new_empty(tuple(t.shape))
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors (non-negative strides) meet."""
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(
+        (n - 1) * s for n, s in zip(t.shape, t.stride())))) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 def launch(fn, t: torch.Tensor, where: str, *args):
     """fn(*args, stream) with t's device current and on its current stream;
     raises on a status other than 0.  The raw getters take 0.1 us where

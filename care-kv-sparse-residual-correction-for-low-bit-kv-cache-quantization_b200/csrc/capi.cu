@@ -478,7 +478,7 @@ int carekv_w4_matvec(const carekv_w4_t* w, const void* x, int64_t x_stride, int3
 static int validate_prefix(const carekv_prefix_t* p, int32_t rows, int32_t heads) {
   if (!p || p->num_kv_heads < 1 || p->tokens < 0 || p->head_dim < 1 || rows < 0 || heads < 1) return CAREKV_ERR_INVALID_ARG;
   if (heads % p->num_kv_heads) return CAREKV_ERR_INVALID_ARG;
-  if (p->head_dim > 256 || p->num_kv_heads > 65535 || static_cast<int64_t>(rows) * heads > INT32_MAX)
+  if (p->head_dim > 256 || p->num_kv_heads > 65535 || p->tokens > (1 << 30) || static_cast<int64_t>(rows) * heads > INT32_MAX)
     return CAREKV_ERR_UNSUPPORTED;
   return validate_dtype(p->dtype);
 }

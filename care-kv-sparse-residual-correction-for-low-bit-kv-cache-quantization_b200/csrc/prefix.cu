@@ -7,7 +7,7 @@
 // Rows of all sequences and the query heads of one kv head form one matrix,
 // so every K / V tile is read once for all of them.  The prefix is split over
 // CTAs; each writes its unnormalised sum, running maximum and weight sum in
-// fp32 and combine_kernel joins them with the rows' own state.
+// fp32 and a second kernel joins them with the rows' own state.
 #include <algorithm>
 
 #include "common.cuh"
@@ -886,7 +886,7 @@ bool tc_split(const carekv_prefix_t& p, int rows, int heads, Split* s) {
   if (tiles <= sms) {
     const int per = s->blocks <= kJoin ? 1 : static_cast<int>(std::min<int64_t>(sms / tiles, s->blocks));
     const int64_t even = (units + sms - 1) / sms;
-    if (per == 1 && s->blocks <= kJoin || (s->blocks + per - 1) / per <= even + kCross) {
+    if (s->blocks <= kJoin || (s->blocks + per - 1) / per <= even + kCross) {
       s->group = s->blocks;
       s->per = per;
       s->ctas = static_cast<int>(tiles) * per;

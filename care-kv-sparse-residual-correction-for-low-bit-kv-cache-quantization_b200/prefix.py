@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._tensors import dtype_code, launch, need_cuda, need_like, new_rows, rows_of
+from ._tensors import dtype_code, launch, need_cuda, need_like, new_rows, overlap, rows_of
 
 
 def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = None,
@@ -69,6 +69,8 @@ def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = N
         need_like(out, q, "prefix_attention out")
         if out.shape != q.shape or not out.is_contiguous():
             raise ValueError(f"prefix_attention out: expected a contiguous tensor of shape {tuple(q.shape)}")
+        if any(overlap(out, t) for t in (q, k, v)):
+            raise ValueError("prefix_attention out: must not overlap q, k or v")
     lse = q.new_empty((n, hq), dtype=torch.float32) if return_lse else None
     k0, k1, _ = k.stride()
     v0, v1, _ = v.stride()

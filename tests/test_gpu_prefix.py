@@ -253,3 +253,36 @@ def test_refusals():
     with pytest.raises(ck._lib.CareKVError, match="unsupported"):
         big = torch.zeros(1, 1, 512, device="cuda")
         ck.prefix_attention(big, big, big)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,hq,hkv,D,N", [
+    (1200, 40, 40, 64, 300),     # more tiles than SMs: whole tiles first, the rest shared
+    (700, 64, 64, 128, 520),
+    (20, 100, 100, 64, 8192),    # tiles do not divide the SMs: CTAs cross from one tile into the next
+    (3, 90, 90, 128, 5000),
+    (5, 148, 148, 64, 640)])     # a tile per SM
+def test_shares_of_the_prefix(dtype, n, hq, hkv, D, N):
+    """Every way the prefix is cut over CTAs, with all tokens seen and with ragged lengths and own states."""
+    ck = pkg()
+    q, k, v = inputs(n, hq, hkv, D, N, dtype, n + hq)
+    o, lse = ck.prefix_attention(q, k, v, return_lse=True)
+    check(o, lse, q, k, v, dtype)
+    g = torch.Generator(device="cuda").manual_seed(N)
+    lengths = torch.randint(0, N + 1, (n,), device="cuda", generator=g, dtype=torch.int32)
+    lengths[0] = 0
+    tail = own_state(n, hq, D, dtype)
+    o, lse = ck.prefix_attention(q, k, v, lengths=lengths, tail=tail, return_lse=True)
+    check(o, lse, q, k, v, dtype, lengths=lengths, tail=tail)
+
+
+def test_result_must_not_overlap_its_inputs():
+    ck = pkg()
+    buf = torch.randn(3, 4, 8, 64, device="cuda", dtype=torch.bfloat16)
+    k = torch.randn(2, 50, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="overlap"):
+        ck.prefix_attention(buf[0], k, k, out=buf[0])
+    want = ck.prefix_attention(buf[0], k, k)
+    assert torch.equal(ck.prefix_attention(buf[0], k, k, out=buf[1]), want)      # neighbours in one buffer are fine
+    none = torch.empty(0, 8, 64, device="cuda", dtype=torch.bfloat16)
+    assert ck.prefix_attention(none, k, k, out=torch.empty_like(none)).shape == (0, 8, 64)

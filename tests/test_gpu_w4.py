@@ -139,3 +139,15 @@ def test_refusals():
     p16, s16, _ = weight(16, 128, 16, "f16")
     with pytest.raises(ck._lib.CareKVError, match="unsupported"):
         ck.PackedWeight(p16, s16, 16)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,k,group,m", [(3001, 2912, 32, 33), (3001, 2912, 32, 64), (2999, 3008, 64, 41),
+                                         (8209, 4128, 32, 17), (8200, 4224, 128, 20), (8193, 4352, 256, 32),
+                                         (8209, 4128, 32, 100)])
+def test_larger_weights_of_odd_sizes(dtype, n, k, group, m):
+    """Weights above the size from which more rows go to the tensor cores: ragged rows, channels, groups, batches."""
+    ck = pkg()
+    packed, scale, w = weight(n, k, group, dtype, n + m)
+    x = torch.randn(m, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(m)).to(DT[dtype])
+    check(ck.PackedWeight(packed, scale, group).matvec(x), x, w, dtype)
