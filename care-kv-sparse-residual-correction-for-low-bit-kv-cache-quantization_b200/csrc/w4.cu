@@ -248,7 +248,9 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int j) { return j == 0 
 // the tiles of the rows in turn and add their sums in shared memory.  The
 // next tile's loads are issued before the present tile's products;
 // activations come through L1.  Column lanes past the last row repeat row 0
-// (their sums are not stored).
+// (their sums are not stored).  Bound by the conversion of the codes (issue)
+// and, in small weights, by the latency of the loads: 1 row x 13824 x 5120
+// 11.1 us, 3.4 TB/s; 1 x 4096 x 4096 4.2 us; 16 rows x 14336 x 4096 18.4 us.
 template <int DT, int NS, int MT, int RT, int WK>
 __global__ void __launch_bounds__(WK * 32) w4_kernel(const typename Act<DT>::T* __restrict__ x, int64_t ldx, int M,
                                                      const uint4* __restrict__ codes,
@@ -380,13 +382,15 @@ __global__ void __launch_bounds__(WK * 32) w4_kernel(const typename Act<DT>::T* 
 // thread multiplies by its scale and adds in fp32 registers: weights stay
 // exact.  Groups of four warps take the tiles in turn, each converting,
 // issuing its products (one warp issuing for all took 0.5 us a tile), waiting
-// for them and adding by itself; what hides the waits is the other groups' work, so there are as many as the registers allow (the NT
-// sums of a row are held by each).  Codes and scales come through shared
+// for them and adding by itself; what hides the waits is the other groups'
+// work, so there are as many as the registers allow (the NT sums of a row are
+// held by each).  Codes and scales come through shared
 // memory too, by bulk copies several tiles ahead: with the two tiles a thread
 // could hold in registers the loads in flight bounded the kernel (5120 rows
-// of 13824 channels, 64 activation rows: 35.5 us instead of 28.6).  The channels are split over the CTAs of a
-// cluster, which add their sums through distributed shared memory in a fixed
-// order.
+// of 13824 channels, 64 activation rows: 35.5 us instead of 28.6, which is
+// 1.4 TB/s or 317 TFLOP/s; bound by a tile's conversion and the wait for its
+// products).  The channels are split over the CTAs of a cluster, which add
+// their sums through distributed shared memory in a fixed order.
 template <int NS, int NT>
 struct TcLayout {
   static constexpr int kStages = NT == 64 ? 6 : 8;

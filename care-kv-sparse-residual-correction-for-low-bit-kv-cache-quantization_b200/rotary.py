@@ -128,8 +128,9 @@ def _check_out(q, k, out):
         need_like(y, q, f"apply_rotary out {what}")
         if y.shape != x.shape or (y.stride(-1) != 1 and x.shape[-1] > 1):
             raise ValueError(f"apply_rotary out {what}: expected shape {tuple(x.shape)} with unit channel stride")
-        held = y.untyped_storage().data_ptr()
-        if held == q.untyped_storage().data_ptr() or (k is not None and held == k.untyped_storage().data_ptr()):
+        held = y.untyped_storage().data_ptr()   # 0 without memory
+        if held and (held == q.untyped_storage().data_ptr()
+                     or (k is not None and held == k.untyped_storage().data_ptr())):
             raise ValueError("apply_rotary out: must not share storage with q or k")
     return yq, yk
 

@@ -14,7 +14,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._tensors import dtype_code, launch, need_cuda, need_like
+from ._tensors import dtype_code, launch, need_cuda, need_like, overlap
 from .quantizer import QuantConfig, pack_codes_2d, quantize
 
 # rows up to which matmul multiplies from the codes (PackedWeight.matmul)
@@ -93,6 +93,8 @@ class PackedWeight:
             need_like(out, x, "matvec out")
             if tuple(out.shape) != (*shape[:-1], n) or not out.is_contiguous():
                 raise ValueError(f"matvec out: expected a contiguous tensor of shape {(*shape[:-1], n)}")
+            if overlap(out, flat):
+                raise ValueError("matvec out: must not overlap x")
         launch(_lib.lib().carekv_w4_matvec, x, "carekv_w4_matvec", self._ref, flat.data_ptr(),
                max(flat.stride(0), k), rows, out.data_ptr())
         return out

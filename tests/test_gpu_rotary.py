@@ -188,3 +188,12 @@ def test_empty_other_stream_and_refusals():
         ck.rotary_frequencies(7)
     with pytest.raises(ValueError, match="original_max_position"):
         ck.rotary_frequencies(8, scaling="yarn", factor=2.0)
+
+
+def test_no_tokens_into_a_given_result():
+    ck = pkg()
+    freq, _ = ck.rotary_frequencies(64, device="cuda")
+    q = torch.empty(0, 4, 64, device="cuda", dtype=torch.float16)
+    y, _ = ck.apply_rotary(q, None, torch.empty(0, device="cuda", dtype=torch.int64), freq,
+                           out=(torch.empty_like(q), None))
+    assert y.shape == q.shape

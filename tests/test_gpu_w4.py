@@ -151,3 +151,16 @@ def test_larger_weights_of_odd_sizes(dtype, n, k, group, m):
     packed, scale, w = weight(n, k, group, dtype, n + m)
     x = torch.randn(m, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(m)).to(DT[dtype])
     check(ck.PackedWeight(packed, scale, group).matvec(x), x, w, dtype)
+
+
+def test_result_must_not_overlap_its_rows():
+    ck = pkg()
+    packed, scale, w = weight(64, 64, 32, "bf16", 3)
+    pw = ck.PackedWeight(packed, scale, 32)
+    buf = torch.randn(2, 5, 64, device="cuda").to(torch.bfloat16)
+    with pytest.raises(ValueError, match="overlap"):
+        pw.matvec(buf[0], out=buf[0])
+    x = buf[0].clone()
+    check(pw.matvec(buf[0], out=buf[1]), x, w, "bf16")       # neighbours in one buffer are fine
+    none = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16)
+    assert pw.matvec(none, out=torch.empty_like(none)).shape == (0, 64)
