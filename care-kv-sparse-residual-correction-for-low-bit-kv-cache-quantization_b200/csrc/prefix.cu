@@ -57,6 +57,7 @@ struct PrefixArgs {
   float* lse;
   float* po;               // unnormalised partial sums [slot][tile row][D]
   float2* ml;              // [slot][tile row]: base-2 maximum, weight sum
+  bool out32;              // out starts on a 32-byte boundary
   Split sp;
 };
 
@@ -254,8 +255,14 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 }
 
 // A whole 32-byte sector per lane: the rows of a warp lie apart, and two
-// 16-byte stores would each write half a sector.
-__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+// 16-byte stores would each write half a sector.  The store wants p on a
+// 32-byte boundary (`aligned`); elsewhere it is two stores of 16 bytes.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8], bool aligned) {
+  if (!aligned) {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    return;
+  }
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
@@ -274,7 +281,7 @@ __device__ __forceinline__ void store_row(const PrefixArgs& a, const Segment& s,
       uint32_t w[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(o[i + j]);
-      store32(a.po + at * D + c0 + i, w);
+      store32(a.po + at * D + c0 + i, w, true);
     }
     return;
   }
@@ -305,7 +312,7 @@ __device__ __forceinline__ void store_row(const PrefixArgs& a, const Segment& s,
         w[4 * g + j] = pack16<BF>(fmaf(wt, f.x, wo * o[c]) * inv, fmaf(wt, f.y, wo * o[c + 1]) * inv);
       }
     }
-    store32(d + 2 * k, w);
+    store32(d + 2 * k, w, a.out32);
   }
 }
 
@@ -980,14 +987,15 @@ cudaError_t launch_combine(const PrefixArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-// room for either form
+// room for either form, and for the partial sums to start on a 32-byte
+// boundary (store32) in a buffer that starts on one of 16
 size_t prefix_workspace_bytes(const carekv_prefix_t& p, int rows, int heads) {
   const size_t row = static_cast<size_t>(p.head_dim + 2) * sizeof(float);
   size_t n = static_cast<size_t>(fma_splits(p, rows, heads)) * rows * heads;
   Split s;
   if (tc_shape(p) && rows > 0 && tc_split(p, rows, heads, &s))
     n = std::max(n, static_cast<size_t>(2) * s.ctas * s.tile_rows);
-  return n * row;
+  return n ? n * row + 16 : 0;
 }
 
 cudaError_t launch_prefix(const carekv_prefix_t& p, const void* q, int64_t q_row, int64_t q_head, int rows, int heads,
@@ -1009,6 +1017,8 @@ cudaError_t launch_prefix(const carekv_prefix_t& p, const void* q, int64_t q_row
   a.tail_lse = tail_lse;
   a.out = out;
   a.lse = lse;
+  a.out32 = (reinterpret_cast<uintptr_t>(out) & 31) == 0;
+  a.po = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(ws) + 31) & ~uintptr_t{31});
   const uintptr_t m = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
                       reinterpret_cast<uintptr_t>(tail) | static_cast<uintptr_t>(q_row * 2) |
                       static_cast<uintptr_t>(q_head * 2);
@@ -1016,7 +1026,6 @@ cudaError_t launch_prefix(const carekv_prefix_t& p, const void* q, int64_t q_row
   int kh, vh;
   if (tc_shape(p) && (m & 15) == 0 && tc_split(p, rows, heads, &a.sp) && tensor_map(&km, p.k, p, p.k_stride, &kh) &&
       tensor_map(&vm, p.v, p, p.v_stride, &vh)) {
-    a.po = static_cast<float*>(ws);
     a.ml = reinterpret_cast<float2*>(a.po + static_cast<size_t>(2) * a.sp.ctas * a.sp.tile_rows * p.head_dim);
     const bool bf = p.dtype == CAREKV_BF16;
     const cudaError_t e = p.head_dim == 128 ? (bf ? launch_tc<128, true>(a, km, vm, kh, vh, st)
@@ -1029,7 +1038,6 @@ cudaError_t launch_prefix(const carekv_prefix_t& p, const void* q, int64_t q_row
     return cut ? launch_combine(a, st) : cudaSuccess;
   }
   const int splits = p.tokens > 0 ? fma_splits(p, rows, heads) : 0;
-  a.po = static_cast<float*>(ws);
   a.ml = reinterpret_cast<float2*>(a.po + static_cast<size_t>(splits) * n * p.head_dim);
   if (splits) {
     const int split_tokens = ((p.tokens + splits - 1) / splits + kFmaTok - 1) / kFmaTok * kFmaTok;

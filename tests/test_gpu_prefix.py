@@ -7,6 +7,7 @@ result is rounded once: |error| <= half ulp |o| + (half ulp + 2 d + 4e-6) sum p 
 The log-sum-exp is off by at most d + 4e-6 (1 + |lse|).
 """
 
+import ctypes
 import math
 
 import pytest
@@ -286,3 +287,33 @@ def test_result_must_not_overlap_its_inputs():
     assert torch.equal(ck.prefix_attention(buf[0], k, k, out=buf[1]), want)      # neighbours in one buffer are fine
     none = torch.empty(0, 8, 64, device="cuda", dtype=torch.bfloat16)
     assert ck.prefix_attention(none, k, k, out=torch.empty_like(none)).shape == (0, 8, 64)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,hq,hkv,D,N", [(1, 4, 4, 64, 300), (40, 8, 2, 128, 512),     # tiles that a CTA holds whole
+                                          (700, 64, 64, 128, 200), (20, 8, 8, 64, 3000)])   # ... with shared ones; shared
+def test_results_and_workspaces_on_16_byte_boundaries(dtype, n, hq, hkv, D, N):
+    """A result, and (through the C entry) a workspace, that starts 16 bytes past a 32-byte boundary: the same bits."""
+    ck = pkg()
+    q, k, v = inputs(n, hq, hkv, D, N, dtype, N)
+    tail = own_state(n, hq, D, dtype)
+    want, want_lse = ck.prefix_attention(q, k, v, tail=tail, return_lse=True)
+    check(want, want_lse, q, k, v, dtype, tail=tail)
+    buf = torch.zeros(8 + q.numel() + 8, device="cuda", dtype=DT[dtype])
+    out = buf[8:8 + q.numel()].view(n, hq, D)
+    assert out.data_ptr() % 32 == 16
+    ck.prefix_attention(q, k, v, tail=tail, out=out)
+    assert torch.equal(out, want) and not buf[:8].any() and not buf[-8:].any()
+    L = ck._lib
+    prefix = L.PREFIX_PACK(k.data_ptr(), v.data_ptr(), N * D, D, N * D, D, hkv, N, D, L.F16 if dtype == "f16" else L.BF16)
+    need = ctypes.c_size_t(0)
+    L.check(L.lib().carekv_prefix_workspace_bytes(prefix, n, hq, ctypes.byref(need)), "workspace")
+    ws = torch.zeros(need.value + 32, device="cuda", dtype=torch.uint8)
+    assert ws.data_ptr() % 32 == 0
+    lse = torch.empty_like(want_lse)
+    L.check(L.lib().carekv_prefix_attention(prefix, q.data_ptr(), hq * D, D, n, hq, 1 / math.sqrt(D), None,
+                                            tail[0].data_ptr(), tail[1].data_ptr(), out.data_ptr(), lse.data_ptr(),
+                                            ws.data_ptr() + 16, need.value, torch.cuda.current_stream().cuda_stream),
+            "prefix")
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    assert not ws[:16].any() and not ws[need.value + 16:].any()
