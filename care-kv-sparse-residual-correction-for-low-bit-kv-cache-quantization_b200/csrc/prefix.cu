@@ -223,12 +223,12 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^y of two values on the FMA pipe, y >= -126 or clamped to it: y = n + f
-// with n the nearest integer (by adding 1.5 2^23), |f| <= 1/2, a degree-4
-// polynomial for 2^f (fitted for the least relative error, 2.6e-6) and n added
-// to its exponent (Cody and Waite's scheme).
+// 2^y of two values on the FMA pipe, 0 below y = -126 (as ex2 has it; hidden
+// tokens come as -inf): y = n + f with n the nearest integer (by adding
+// 1.5 2^23), |f| <= 1/2, a degree-4 polynomial for 2^f (fitted for the least
+// relative error, 2.6e-6) and n added to its exponent (Cody and Waite's
+// scheme).
 __device__ __forceinline__ float2 ex2_fma(float2 y) {
-  y = make_float2(fmaxf(y.x, -126.f), fmaxf(y.y, -126.f));
   const float2 big = make_float2(12582912.f, 12582912.f), nbig = make_float2(-12582912.f, -12582912.f);
   const float2 r = add2(y, big), n = add2(r, nbig);
   const float2 f = fma2(n, make_float2(-1.f, -1.f), y);
@@ -236,8 +236,8 @@ __device__ __forceinline__ float2 ex2_fma(float2 y) {
   p = fma2(p, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
   p = fma2(p, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
   p = fma2(p, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
+  return make_float2(y.x < -126.f ? 0.f : __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)),
+                     y.y < -126.f ? 0.f : __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
 }
 __device__ __forceinline__ float max_nan(float x, float y) {   // NaN if either is
   float r;
@@ -662,8 +662,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
           __syncwarp();
           if (lane == 0) mbar_arrive((c == 0 ? p_half : p_full) + st);
         }
-        // a row that has seen nothing has no weight (ex2_fma's least is 2^-126)
-        if (m != -INFINITY) l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
       const Segment done_s = s;
       const int done_rho = rho;

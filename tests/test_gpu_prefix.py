@@ -317,3 +317,34 @@ def test_results_and_workspaces_on_16_byte_boundaries(dtype, n, hq, hkv, D, N):
             "prefix")
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
     assert not ws[:16].any() and not ws[need.value + 16:].any()
+
+
+@pytest.mark.parametrize("n,hq,hkv,D,N", [(9, 4, 4, 64, 300), (9, 4, 4, 128, 4000), (300, 2, 2, 64, 700),
+                                          (300, 2, 2, 128, 260)])
+def test_hidden_tokens_weigh_nothing(n, hq, hkv, D, N):
+    """The type's largest values in tokens that a row does not see leave no trace in it."""
+    ck = pkg()
+    q, k, v = inputs(n, hq, hkv, D, N, "bf16", 11)
+    half = N // 2 + 3
+    lengths = torch.full((n,), half, dtype=torch.int32, device="cuda")
+    lengths[1::2] = N
+    clean = v.clone()
+    v[:, half:] = torch.finfo(torch.bfloat16).max / N
+    v[:, half:, ::2] *= -1
+    o, lse = ck.prefix_attention(q, k, v, lengths=lengths, return_lse=True)
+    some = torch.arange(0, n, 2, device="cuda")
+    check(o[some], lse[some], q[some], k, clean, "bf16", lengths=lengths[some])
+
+
+def test_far_scores_weigh_nothing():
+    """Visible tokens whose weight is below 2^-150 of the largest one's leave no trace, whatever their values."""
+    ck = pkg()
+    for n, hq in ((5, 4), (300, 2)):
+        D, N = 64, 256
+        q, k, v = inputs(n, hq, hq, D, N, "bf16", 12, outliers=False)
+        q[..., 0], k[..., 0] = 1.0, 0.0
+        k[:, 1::2, 0] = -1000.0
+        v[:, 1::2] = 1e38
+        o, lse = ck.prefix_attention(q, k, v, scale=1.0, return_lse=True)
+        v[:, 1::2] = 0
+        check(o, lse, q, k, v, "bf16", scale=1.0)
