@@ -75,7 +75,8 @@ def apply_rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, freq: Tensor
     k [B, T, Hkv, D] with positions [B, T] or [T]; any strides (transposed
     views are read in place), positions int32 or int64 of any sign, k may be
     None.  inverse turns back: it maps gradients of the results to gradients
-    of the inputs, which is also what autograd gets.  out = (q_out, k_out):
+    of the inputs, which is also what autograd gets (reverse mode, any order;
+    forward mode and torch.func are not supported).  out = (q_out, k_out):
     tensors of the same shapes to write to (any strides with unit channel
     stride, apart from the inputs), new contiguous ones otherwise.
     """
@@ -89,19 +90,15 @@ def apply_rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, freq: Tensor
 class _Turn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, freq, layout, attention_factor, inverse):
-        ctx.args = (positions, freq, layout, attention_factor, not inverse)
-        ctx.shapes = (q.shape, None if k is None else k.shape)
+        # saved this way, a change of the positions before backward is an error
+        ctx.save_for_backward(positions, freq)
+        ctx.args = (layout, attention_factor, not inverse)
         return _turn(q, k, positions, freq, layout, attention_factor, inverse, None)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        qs, ks = ctx.shapes
-        like = dq if dq is not None else dk
-        if dq is None:
-            dq = like.new_zeros(qs)
-        if dk is None and ks is not None:
-            dk = like.new_zeros(ks)
-        return (*_turn(dq, dk, *ctx.args, None), None, None, None, None, None)
+        # gradients of results that took no part come as zeros; differentiable again
+        return (*apply_rotary(dq, dk, *ctx.saved_tensors, *ctx.args), None, None, None, None, None)
 
 
 _NO_ROWS = (0, 0, 0, 0, 0, 0, 0, 0, 0)   # no tensor, no heads

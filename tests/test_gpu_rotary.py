@@ -197,3 +197,32 @@ def test_no_tokens_into_a_given_result():
     y, _ = ck.apply_rotary(q, None, torch.empty(0, device="cuda", dtype=torch.int64), freq,
                            out=(torch.empty_like(q), None))
     assert y.shape == q.shape
+
+
+def test_positions_changed_before_backward():
+    """A gradient belongs to the positions and frequencies of its forward pass: changing them in place is an error."""
+    ck = pkg()
+    freq, _ = ck.rotary_frequencies(16, device="cuda")
+    for changed in ("positions", "freq"):
+        q = torch.randn(5, 2, 16, device="cuda", requires_grad=True)
+        pos, f = torch.arange(5, device="cuda"), freq.clone()
+        y, _ = ck.apply_rotary(q, None, pos, f)
+        (pos if changed == "positions" else f).add_(1)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.sum().backward()
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_second_derivative(layout):
+    """The gradient is linear in the output's gradient and can be differentiated by it: the forward turn again."""
+    ck = pkg()
+    freq, _ = ck.rotary_frequencies(12, device="cuda")
+    pos = torch.arange(4, device="cuda") * 31
+    q = torch.randn(4, 3, 16, device="cuda", requires_grad=True)
+    w = torch.randn(4, 3, 16, device="cuda", requires_grad=True)
+    u = torch.randn(4, 3, 16, device="cuda")
+    y, _ = ck.apply_rotary(q, None, pos, freq, layout=layout, attention_factor=1.25)
+    (dq,) = torch.autograd.grad((y * w).sum(), q, create_graph=True)
+    check(dq.detach(), w.detach(), pos, freq, layout, 1.25, True, "f32")
+    (dw,) = torch.autograd.grad((dq * u).sum(), w)
+    check(dw, u, pos, freq, layout, 1.25, False, "f32")
