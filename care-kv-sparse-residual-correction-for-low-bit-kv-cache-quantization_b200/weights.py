@@ -67,7 +67,16 @@ class PackedWeight:
 
     def matvec(self, x: Tensor, out: Optional[Tensor] = None) -> Tensor:
         """x [..., K] @ weight^T -> [..., N] in x's dtype (the scales' dtype),
-        read from the codes: made for the few rows of a decode step."""
+        read from the codes: made for the few rows of a decode step.
+        Differentiable in x (without out): its gradient is a dense product
+        with the dequantized weight."""
+        if x.requires_grad and torch.is_grad_enabled():
+            if out is not None:
+                raise RuntimeError("matvec: out= does not take part in autograd")
+            return _Product.apply(x, self.codes, self.scales, self)
+        return self._matvec(x, out)
+
+    def _matvec(self, x: Tensor, out: Optional[Tensor]) -> Tensor:
         n, k = self.shape
         if x.get_device() != self._index:
             raise RuntimeError(f"matvec x: expected a tensor on {self.device}, got {x.device}")
@@ -112,3 +121,16 @@ class PackedWeight:
         if x.numel() <= MATVEC_ROWS * self.shape[1]:
             return self.matvec(x)
         return x @ self.dequantize().t()
+
+
+class _Product(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, codes, scales, weight):
+        ctx.save_for_backward(codes, scales)   # a weight changed before backward is an error
+        ctx.weight = weight
+        return weight._matvec(x, None)
+
+    @staticmethod
+    def backward(ctx, dy):
+        ctx.saved_tensors
+        return dy @ ctx.weight.dequantize(), None, None, None

@@ -164,3 +164,51 @@ def test_result_must_not_overlap_its_rows():
     check(pw.matvec(buf[0], out=buf[1]), x, w, "bf16")       # neighbours in one buffer are fine
     none = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16)
     assert pw.matvec(none, out=torch.empty_like(none)).shape == (0, 64)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 64, 65])
+def test_gradient_of_the_activations(dtype, rows):
+    """dx = dy W, on both sides of the row limit of matmul.  Tolerance: the weight rounded to the dtype (half an ulp of
+    each term), the library product's sums (n 2^-24, and half an ulp where a partial sum is kept in the dtype) and the
+    result's own rounding."""
+    ck = pkg()
+    n, k = 96, 160
+    packed, scale, w = weight(n, k, 32, dtype, 21)
+    pw = ck.PackedWeight(packed, scale, 32)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    plain = torch.randn(rows, k, device="cuda", generator=g).to(DT[dtype])
+    dy = torch.randn(rows, n, device="cuda", generator=g).to(DT[dtype])
+    ref, size = dy.double() @ w, dy.double().abs() @ w.abs()
+    tol = HALF_ULP[dtype] * (ref.abs() + 2 * size) + n * 2.0 ** -24 * size + (2.0 ** -24 if dtype == "f16" else 0.0)
+    for fn in (pw.matvec, pw.matmul):
+        x = plain.clone().requires_grad_()
+        y = fn(x)
+        assert y.requires_grad and torch.equal(y.detach(), fn(plain))
+        y.backward(dy)
+        assert x.grad.dtype == x.dtype and bool(((x.grad.double() - ref).abs() <= tol).all())
+    x = plain.clone().requires_grad_()
+    y = pw.matvec(x[None])
+    y.backward(dy[None])
+    assert bool(((x.grad.double() - ref).abs() <= tol).all())
+    with pytest.raises(RuntimeError, match="autograd"):
+        pw.matvec(x, out=torch.empty(rows, n, device="cuda", dtype=x.dtype))
+    with torch.no_grad():
+        assert not pw.matvec(x).requires_grad
+
+
+def test_gradient_against_differences():
+    """The map is linear: a central difference is the gradient up to rounding (fp32 sums of 64 products below 1)."""
+    ck = pkg()
+    packed, scale, w = weight(16, 64, 32, "f32", 22)
+    pw = ck.PackedWeight(packed, scale, 32)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(2, 64, device="cuda", generator=g, requires_grad=True)
+    dy = torch.randn(2, 16, device="cuda", generator=g)
+    pw.matvec(x).backward(dy)
+    for j in (0, 31, 32, 63):
+        e = torch.zeros_like(x)
+        e[1, j] = 0.5
+        with torch.no_grad():
+            diff = float(((pw.matvec(x + e) - pw.matvec(x - e)).double() * dy.double()).sum())
+        assert diff == pytest.approx(float(x.grad[1, j]), abs=1e-3)
