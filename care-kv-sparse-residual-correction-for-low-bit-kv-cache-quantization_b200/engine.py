@@ -161,7 +161,8 @@ class DecodeEngine:
         result (its residual correction routed over the own tokens alone) is
         merged with attention over the prefix of this layer (same dtype and
         kv heads as the cache's).
-        return_lse: also the fp32 log-sum-exp [seq_count, Hq] of the attention."""
+        return_lse: also the fp32 log-sum-exp [seq_count, Hq] of the attention.
+        The results carry no graph."""
         cfg = self.cfg
         n = q.shape[0]
         q = self._check_tensor(q, (n, self.kvh_total * self.qn, cfg.head_dim), "decode q")
@@ -185,6 +186,7 @@ class DecodeEngine:
             self._sketch_ptr(), ws.data_ptr(), ws.numel(), ctypes.byref(self.shard), self._stream()),
             "carekv_decode_attention")
         if prefix is not None:
+            q = q.detach()
             h0, h1 = self.shard.kvh_begin * self.qn, (self.shard.kvh_begin + cfg.num_kv_heads) * self.qn
             if h1 - h0 == q.shape[1]:
                 _, lse = prefix.attend(layer, q, tail=(own, lse), out=out, return_lse=True)

@@ -35,7 +35,10 @@ def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = N
     Returns [n, Hq, D] in q's dtype, with return_lse also the merged
     log-sum-exp [n, Hq] fp32; a row that sees nothing gives 0 and -inf.
     Values of a token that any row sees must be finite for every row.
+    There is no backward pass: inputs that require a gradient are refused.
     """
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ((q, k, v) if tail is None else (q, k, v, *tail))):
+        raise RuntimeError("prefix_attention has no backward pass: detach its inputs or call it under no_grad")
     need_cuda(q, "prefix_attention q")
     dt = dtype_code(q, "prefix_attention q")
     if q.dim() != 3 or k.dim() != 3:

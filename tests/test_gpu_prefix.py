@@ -348,3 +348,21 @@ def test_far_scores_weigh_nothing():
         o, lse = ck.prefix_attention(q, k, v, scale=1.0, return_lse=True)
         v[:, 1::2] = 0
         check(o, lse, q, k, v, "bf16", scale=1.0)
+
+
+def test_inputs_that_require_a_gradient_are_refused():
+    """The operator has no backward pass: it says so instead of dropping a gradient."""
+    ck = pkg()
+    q, k, v = inputs(3, 4, 2, 64, 40, "f32")
+    tail = own_state(3, 4, 64, "f32")
+    args = dict(q=q, k=k, v=v)
+    for name in args:
+        bad = dict(args, **{name: args[name].clone().requires_grad_()})
+        with pytest.raises(RuntimeError, match="backward"):
+            ck.prefix_attention(**bad)
+        with torch.no_grad():
+            assert torch.equal(ck.prefix_attention(**bad), ck.prefix_attention(q, k, v))
+    for i in range(2):
+        bad = tuple(t.clone().requires_grad_() if j == i else t for j, t in enumerate(tail))
+        with pytest.raises(RuntimeError, match="backward"):
+            ck.prefix_attention(q, k, v, tail=bad)

@@ -250,3 +250,16 @@ def test_layer_refusals(pkg):
             layer.prefill_batch(cache, hid, positions=torch.arange(5, device="cuda"))
         with pytest.raises(ValueError, match="has not been set"):
             pkg.SharedPrefix(1).attend(0, torch.randn(1, 2, 64, device="cuda"))
+
+
+def test_decode_attention_carries_no_graph(pkg):
+    """attend() answers alike whether its queries require a gradient, with and without a prefix."""
+    with env(**PAPER_BEST_ENV):
+        cfg, cache, eng, seqs, q = build(pkg, 64, 3, 32, 4, 2, "fp32", (20, 5), 3, read_budget_mode="absolute",
+                                         read_abs_k=1, read_abs_v=1)
+        sp = pkg.SharedPrefix(1)
+        sp.set(0, torch.randn(2, 50, 64, device="cuda"), torch.randn(2, 50, 64, device="cuda"))
+        qt = torch.from_numpy(q).cuda()
+        for kw in ({}, dict(prefix=sp)):
+            got = eng.attend(0, qt.clone().requires_grad_(), **kw)
+            assert not got.requires_grad and torch.equal(got, eng.attend(0, qt, **kw))
