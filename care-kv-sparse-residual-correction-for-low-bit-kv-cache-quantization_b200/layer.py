@@ -158,6 +158,9 @@ class CAREKVLayer(nn.Module):
             raise ValueError("positions need layer.rotary (a RotaryEmbedding)")
         if position_embeddings is not None:
             raise ValueError("position_embeddings or positions, not both")
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+            yq, yk = self.rotary(q.transpose(1, 2), k.transpose(1, 2), positions)
+            return yq.transpose(1, 2), yk.transpose(1, 2)
         yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
         self.rotary(q.transpose(1, 2), k.transpose(1, 2), positions,
                     out=(yq.transpose(1, 2), yk.transpose(1, 2)))
@@ -204,6 +207,8 @@ class CAREKVLayer(nn.Module):
         B, T, _ = hidden.shape
         g = cfg.num_heads // cfg.num_kv_heads
         q, k, v = self._project(hidden)
+        if prefix is not None and torch.is_grad_enabled() and (q.requires_grad or v.requires_grad):
+            raise RuntimeError("prefill with a prefix has no backward pass: call it under no_grad")
         q_post, k_post = self._rotate(q, k, position_embeddings, positions)
         eng = engine_for(cache)
         eng.prefill_store(self.layer_id, k_post.contiguous(), v.contiguous(), seq_begin=seq_begin,

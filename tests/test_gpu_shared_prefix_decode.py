@@ -263,3 +263,43 @@ def test_decode_attention_carries_no_graph(pkg):
         for kw in ({}, dict(prefix=sp)):
             got = eng.attend(0, qt.clone().requires_grad_(), **kw)
             assert not got.requires_grad and torch.equal(got, eng.attend(0, qt, **kw))
+
+
+def test_layer_calls_with_inputs_that_require_a_gradient(pkg):
+    """Prefill by positions passes the gradient that prefill by tables passes; with a prefix, whose attention has no
+    backward pass, it refuses.  Decode steps answer as without a gradient, as they do without positions or a prefix."""
+    with env(CAREKV_PREFILL_MODE="fp", **PAPER_BEST_ENV):
+        Hq, Hkv, D, dm, N, T = 4, 2, 64, 96, 40, 9
+        cfg = pkg.CacheConfig(num_layers=1, num_heads=Hq, num_kv_heads=Hkv, head_dim=D, max_pages=4, base_bits=4,
+                              group_size=32, scale_quant="int8", packed_base=True, store_budget_mode="absolute",
+                              store_abs_k=1, store_abs_v=1, read_budget_mode="absolute", read_abs_k=1, read_abs_v=1,
+                              route_policy="joint", store_sketch=False)
+        g = torch.Generator(device="cuda").manual_seed(3)
+        ws = [torch.randn(o, i, device="cuda", generator=g) / math.sqrt(i)
+              for o, i in ((Hq * D, dm), (Hkv * D, dm), (Hkv * D, dm), (dm, Hq * D))]
+        layer = pkg.CAREKVLayer(cfg, 0, *ws, torch.device("cuda"))
+        layer.rotary = pkg.RotaryEmbedding(D, device="cuda")
+        sp = pkg.SharedPrefix(1)
+        sp.set(0, *(torch.randn(Hkv, N, D, device="cuda", generator=g) for _ in range(2)))
+        hid = torch.randn(1, T, dm, device="cuda", generator=g)
+        pos = torch.arange(T, device="cuda")
+        ang = pos.double().unsqueeze(-1) * (layer.rotary.freq.double() * (2 * math.pi / 2.0 ** 64))
+        tables = tuple(torch.cat((f(ang), f(ang)), -1).float()[None] for f in (torch.cos, torch.sin))
+        grads = []
+        for kw in (dict(position_embeddings=tables), dict(positions=pos)):
+            x = hid.clone().requires_grad_()
+            cache = pkg.CAREKVCache(cfg, torch.device("cuda"), batch=1)
+            layer.prefill_batch(cache, x, **kw).square().sum().backward()
+            grads.append(x.grad)
+        torch.testing.assert_close(grads[1], grads[0], rtol=1e-3, atol=1e-3 * float(grads[0].abs().max()))
+        x = hid.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="backward"):
+            layer.prefill_batch(pkg.CAREKVCache(cfg, torch.device("cuda"), batch=1), x, positions=N + pos, prefix=sp)
+        outs = []
+        for grad in (False, True):
+            cache = pkg.CAREKVCache(cfg, torch.device("cuda"), batch=1)
+            with torch.no_grad():
+                layer.prefill_batch(cache, hid, positions=N + pos, prefix=sp)
+            step = hid[:, 0].clone().requires_grad_(grad)
+            outs.append(layer.decode_step_batch(cache, step, positions=N + pos[-1:] + 1, prefix=sp))
+        assert torch.equal(outs[0], outs[1])
