@@ -122,21 +122,22 @@ class CAREKVLayer(nn.Module):
         self.W_O = nn.Parameter(W_O, requires_grad=False)
         self.base_qcfg = QuantConfig(bits=cfg.base_bits, group_size=cfg.group_size)
         self.rotary: Optional[RotaryEmbedding] = None
-        self._packed: Dict[str, PackedWeight] = {}
+        self._packed = nn.ModuleDict()   # 4-bit weights in place of the parameters of these names
 
     def quantize_weights(self, group_size: int = 32) -> "CAREKVLayer":
         """Replace the projections by 4-bit weights with one scale per
         `group_size` input channels (the package quantizer's codes)."""
-        for name in ("W_Q", "W_K", "W_V", "W_O"):
-            if name not in self._packed:
-                self._packed[name] = PackedWeight.from_dense(getattr(self, name).data, group_size)
-                setattr(self, name, None)
+        packed = {name: PackedWeight.from_dense(getattr(self, name).data, group_size)
+                  for name in ("W_Q", "W_K", "W_V", "W_O") if name not in self._packed}
+        for name, w in packed.items():
+            self._packed[name] = w
+            setattr(self, name, None)
         return self
 
     def _linear(self, name: str, x: Tensor) -> Tensor:
         """x [..., K] @ W^T with the dense or the 4-bit weight."""
-        w = self._packed.get(name)
-        return x @ getattr(self, name).T if w is None else w.matmul(x)
+        w = getattr(self, name)
+        return self._packed[name].matmul(x) if w is None else x @ w.T
 
     # ── projections ──────────────────────────────────────────────────
     def _project(self, hidden: Tensor):

@@ -14,7 +14,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch import Tensor
+from torch import Tensor, nn
 
 from . import _lib
 from ._tensors import dtype_code, launch, need_cuda, need_like, new_rows, rows_of
@@ -183,16 +183,19 @@ def _turn(q, k, positions, freq, layout, attention_factor, inverse, out):
     return yq, yk
 
 
-class RotaryEmbedding:
-    """Frequencies and layout of a model's rotary positions, kept on the device."""
+class RotaryEmbedding(nn.Module):
+    """Frequencies and layout of a model's rotary positions, kept on the device
+    (a buffer that moves with the module and stays out of state dicts)."""
 
     def __init__(self, rotary_dim: int, base: float = 10000.0, layout: str = "half", scaling: str = "none",
                  factor: float = 1.0, original_max_position: Optional[int] = None, device="cuda"):
         if layout not in LAYOUTS:
             raise ValueError(f"layout={layout}: half or interleaved")
+        super().__init__()
         self.layout = layout
-        self.freq, self.attention_factor = rotary_frequencies(
-            rotary_dim, base, scaling, factor, original_max_position, device=device)
+        freq, self.attention_factor = rotary_frequencies(rotary_dim, base, scaling, factor, original_max_position,
+                                                         device=device)
+        self.register_buffer("freq", freq, persistent=False)
 
-    def __call__(self, q: Tensor, k: Optional[Tensor], positions: Tensor, inverse: bool = False, out=None):
+    def forward(self, q: Tensor, k: Optional[Tensor], positions: Tensor, inverse: bool = False, out=None):
         return apply_rotary(q, k, positions, self.freq, self.layout, self.attention_factor, inverse, out)

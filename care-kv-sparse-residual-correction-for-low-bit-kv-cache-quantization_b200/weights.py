@@ -11,22 +11,25 @@ import ctypes
 from typing import Optional
 
 import torch
-from torch import Tensor
+from torch import Tensor, nn
 
 from . import _lib
-from ._tensors import dtype_code, launch, need_cuda, need_like, overlap
+from ._tensors import DT, dtype_code, launch, need_cuda, need_like, overlap
 from .quantizer import QuantConfig, pack_codes_2d, quantize
 
 # rows up to which matmul multiplies from the codes (PackedWeight.matmul)
 MATVEC_ROWS = 64
 
 
-class PackedWeight:
+class PackedWeight(nn.Module):
     """Weight [N, K] as 4-bit codes -8..7 times one scale per `group_size`
     channels of a row.  packed [N, K/2]: rows of ``pack_int4_2d``; scale
-    [N, K/group_size] in the activations' dtype."""
+    [N, K/group_size] in the activations' dtype.  Codes and scales are byte
+    buffers of the module, so state dicts hold them, copies and moves between
+    devices keep them, and no cast changes them."""
 
     def __init__(self, packed: Tensor, scale: Tensor, group_size: int):
+        super().__init__()
         need_cuda(packed, "PackedWeight packed")
         need_cuda(scale, "PackedWeight scale")
         if packed.dtype not in (torch.uint8, torch.int8) or packed.dim() != 2:
@@ -42,19 +45,51 @@ class PackedWeight:
         self.shape = (n, k)
         self.group_size = group_size
         self.dtype = scale.dtype
-        self.device = packed.device
-        self.c = _lib.W4()
-        self.c.n, self.c.k, self.c.group_size = n, k, group_size
-        self.c.dtype = dtype_code(scale, "PackedWeight scale")
+        c = _lib.W4(n=n, k=k, group_size=group_size, dtype=dtype_code(scale, "PackedWeight scale"))
         sizes = (ctypes.c_size_t * 2)()
         lib = _lib.lib()
-        _lib.check(lib.carekv_w4_layout(ctypes.byref(self.c), sizes), "carekv_w4_layout")
-        self.codes = torch.empty(sizes[0], dtype=torch.uint8, device=packed.device)
-        self.scales = torch.empty(sizes[1], dtype=torch.uint8, device=packed.device)
-        self.c.codes, self.c.scales = self.codes.data_ptr(), self.scales.data_ptr()
-        self._ref, self._index = ctypes.byref(self.c), packed.get_device()
-        launch(lib.carekv_w4_pack, packed, "carekv_w4_pack", ctypes.byref(self.c), packed.data_ptr(),
-               scale.data_ptr())
+        _lib.check(lib.carekv_w4_layout(ctypes.byref(c), sizes), "carekv_w4_layout")
+        self.register_buffer("codes", torch.empty(sizes[0], dtype=torch.uint8, device=packed.device))
+        self.register_buffer("scales", torch.empty(sizes[1], dtype=torch.uint8, device=packed.device))
+        self._bind()
+        launch(lib.carekv_w4_pack, packed, "carekv_w4_pack", self._ref, packed.data_ptr(), scale.data_ptr())
+
+    def _bind(self):
+        """The C structure of the buffers as they lie now; no device index off the GPU."""
+        n, k = self.shape
+        self.c = _lib.W4(self.codes.data_ptr(), self.scales.data_ptr(), n, k, self.group_size, DT[self.dtype])
+        self._ref = ctypes.byref(self.c)
+        self.device = self.codes.device
+        self._index = self.codes.get_device() if self.codes.is_cuda and self.scales.device == self.device else None
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self._bind()
+        return self
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("c", "_ref")}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._bind()
+
+    # What the bytes of a state dict stand for: another weight's may be as long.
+    def get_extra_state(self):
+        return dict(layout=1, shape=tuple(self.shape), group_size=self.group_size, dtype=str(self.dtype))
+
+    def set_extra_state(self, state):
+        pass   # compared before the buffers are read
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                              error_msgs):
+        held = state_dict.get(prefix + "_extra_state")
+        if prefix + "codes" in state_dict and held != self.get_extra_state():
+            error_msgs.append(f"PackedWeight {prefix}: expected {self.get_extra_state()}, got {held}")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                                      error_msgs)
+        self._bind()
 
     @classmethod
     def from_dense(cls, weight: Tensor, group_size: int = 32) -> "PackedWeight":
@@ -79,6 +114,7 @@ class PackedWeight:
     def _matvec(self, x: Tensor, out: Optional[Tensor]) -> Tensor:
         n, k = self.shape
         if x.get_device() != self._index:
+            need_cuda(self.codes, "PackedWeight")
             raise RuntimeError(f"matvec x: expected a tensor on {self.device}, got {x.device}")
         if x.dtype is not self.dtype:
             raise ValueError(f"matvec x: expected {self.dtype}, got {x.dtype}")
@@ -110,6 +146,7 @@ class PackedWeight:
 
     def dequantize(self) -> Tensor:
         """The dense weight [N, K], codes * scale rounded to the scales' dtype."""
+        need_cuda(self.codes, "PackedWeight")
         out = torch.empty(self.shape, dtype=self.dtype, device=self.device)
         launch(_lib.lib().carekv_w4_dequantize, out, "carekv_w4_dequantize", self._ref, out.data_ptr())
         return out

@@ -303,3 +303,47 @@ def test_layer_calls_with_inputs_that_require_a_gradient(pkg):
             step = hid[:, 0].clone().requires_grad_(grad)
             outs.append(layer.decode_step_batch(cache, step, positions=N + pos[-1:] + 1, prefix=sp))
         assert torch.equal(outs[0], outs[1])
+
+
+def test_quantized_layer_is_copied_saved_and_moved(pkg):
+    """quantize_weights() loses nothing: a state_dict holds the 4-bit weights, copies and moves keep them, and a layer
+    whose weights cannot all be quantized stays as it was."""
+    import copy
+    Hq, Hkv, D, dm = 4, 2, 64, 96
+    cfg = pkg.CacheConfig(num_layers=1, num_heads=Hq, num_kv_heads=Hkv, head_dim=D, max_pages=4, base_bits=4,
+                          group_size=32, scale_quant="int8", packed_base=True, store_budget_mode="absolute",
+                          store_abs_k=1, store_abs_v=1, read_budget_mode="absolute", read_abs_k=1, read_abs_v=1,
+                          route_policy="joint", store_sketch=False)
+    g = torch.Generator(device="cuda").manual_seed(4)
+
+    def make(out=dm):
+        ws = [torch.randn(o, i, device="cuda", generator=g) / math.sqrt(i)
+              for o, i in ((Hq * D, dm), (Hkv * D, dm), (Hkv * D, dm), (out, Hq * D))]
+        return pkg.CAREKVLayer(cfg, 0, *ws, torch.device("cuda"))
+    layer = make().quantize_weights(32)
+    layer.rotary = pkg.RotaryEmbedding(D, device="cuda")
+    hid = torch.randn(1, 6, dm, device="cuda", generator=g)
+    pos = torch.arange(6, device="cuda")
+
+    def run(l):
+        with env(CAREKV_PREFILL_MODE="fp", **PAPER_BEST_ENV):
+            return l.prefill_batch(pkg.CAREKVCache(cfg, torch.device("cuda"), batch=1), hid, positions=pos)
+    want = run(layer)
+    assert torch.equal(run(copy.deepcopy(layer)), want)
+    state = copy.deepcopy(layer.state_dict())
+    other = make().quantize_weights(32)
+    other.rotary = layer.rotary
+    assert not torch.equal(run(other), want)
+    other.load_state_dict(state)
+    assert torch.equal(run(other), want)
+    moved = copy.deepcopy(layer).cpu()
+    assert moved.rotary.freq.device.type == "cpu"
+    assert torch.equal(run(moved.cuda()), want)
+    assert torch.equal(run(layer), want)
+    odd = make()
+    odd.W_O = torch.nn.Parameter(torch.randn(dm, Hq * D + 16, device="cuda"), requires_grad=False)
+    with pytest.raises(Exception):
+        odd.quantize_weights(32)
+    assert all(getattr(odd, n) is not None for n in ("W_Q", "W_K", "W_V", "W_O"))
+    dense = make()
+    assert set(dense.state_dict()) == {"W_Q", "W_K", "W_V", "W_O"}

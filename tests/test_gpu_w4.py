@@ -212,3 +212,40 @@ def test_gradient_against_differences():
         with torch.no_grad():
             diff = float(((pw.matvec(x + e) - pw.matvec(x - e)).double() * dy.double()).sum())
         assert diff == pytest.approx(float(x.grad[1, j]), abs=1e-3)
+
+
+def test_copies_and_checkpoints():
+    """deepcopy, pickle, .to() and a state_dict keep the weight; a state of another weight is refused."""
+    import copy
+    import io
+    ck = pkg()
+    g = torch.Generator(device="cuda").manual_seed(30)
+    packed, scale, w = weight(40, 96, 32, "f16", 30)
+    pw = ck.PackedWeight(packed, scale, 32)
+    x = torch.randn(3, 96, device="cuda", generator=g).half()
+    want = pw.matvec(x)
+    twin = copy.deepcopy(pw)
+    assert twin.codes.data_ptr() != pw.codes.data_ptr() and torch.equal(twin.matvec(x), want)
+    buf = io.BytesIO()
+    torch.save(pw, buf)
+    buf.seek(0)
+    assert torch.equal(torch.load(buf, weights_only=False).matvec(x), want)
+    state = {k: v.clone() if torch.is_tensor(v) else v for k, v in pw.state_dict().items()}
+    for assign in (False, True):
+        other = ck.PackedWeight(*weight(40, 96, 32, "f16", 31)[:2], 32)
+        assert not torch.equal(other.matvec(x), want)
+        other.load_state_dict({k: v.clone() if torch.is_tensor(v) else v for k, v in state.items()}, assign=assign)
+        assert torch.equal(other.matvec(x), want)
+    for bad in (ck.PackedWeight(*weight(40, 96, 32, "bf16", 31)[:2], 32),     # as many bytes, other values
+                ck.PackedWeight(*weight(48, 96, 32, "f16", 31)[:2], 32)):
+        with pytest.raises((RuntimeError, ValueError), match="PackedWeight"):
+            bad.load_state_dict(state)
+    away = copy.deepcopy(pw).cpu()
+    with pytest.raises(RuntimeError, match="CUDA|expected a tensor on"):
+        away.matvec(x)
+    with pytest.raises(RuntimeError, match="CUDA|expected a tensor on"):
+        away.matvec(x.cpu())
+    with pytest.raises(RuntimeError, match="CUDA|expected a tensor on"):
+        away.dequantize()
+    assert torch.equal(away.cuda().matvec(x), want)
+    assert torch.equal(copy.deepcopy(pw).bfloat16().matvec(x), want)      # codes and scales are bytes: no cast
