@@ -32,6 +32,8 @@ def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = N
     [n] int32: row r sees the prefix tokens below lengths[r] (clamped to
     0..N).  tail = (o [n, Hq, D], lse [n, Hq] fp32): attention output and
     natural log-sum-exp of the row's own tokens, -inf where it has none.
+    out: a contiguous tensor to write to that overlaps no input, but may be
+    tail's o itself.
     Returns [n, Hq, D] in q's dtype, with return_lse also the merged
     log-sum-exp [n, Hq] fp32; a row that sees nothing gives 0 and -inf.
     Values of a token that any row sees must be finite for every row.
@@ -72,8 +74,12 @@ def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = N
         need_like(out, q, "prefix_attention out")
         if out.shape != q.shape or not out.is_contiguous():
             raise ValueError(f"prefix_attention out: expected a contiguous tensor of shape {tuple(q.shape)}")
-        if any(overlap(out, t) for t in (q, k, v)):
-            raise ValueError("prefix_attention out: must not overlap q, k or v")
+        # a row's own state is read by the threads that write the row: in place is fine
+        others = [t for t in (q, k, v, lengths, tail_lse) if t is not None]
+        if tail_o is not None and tail_o.data_ptr() != out.data_ptr():
+            others.append(tail_o)
+        if any(overlap(out, t) for t in others):
+            raise ValueError("prefix_attention out: must not overlap its inputs (but may be the own state's output)")
     lse = q.new_empty((n, hq), dtype=torch.float32) if return_lse else None
     k0, k1, _ = k.stride()
     v0, v1, _ = v.stride()

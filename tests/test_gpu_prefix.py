@@ -366,3 +366,28 @@ def test_inputs_that_require_a_gradient_are_refused():
         bad = tuple(t.clone().requires_grad_() if j == i else t for j, t in enumerate(tail))
         with pytest.raises(RuntimeError, match="backward"):
             ck.prefix_attention(q, k, v, tail=bad)
+
+
+def test_result_over_the_own_state():
+    """`out` may be the own state's output itself; at another place over it, its log-sum-exp or the lengths it is refused."""
+    ck = pkg()
+    for n, N in ((6, 200), (6, 3000), (300, 700)):      # whole tiles, shared tiles, both
+        q, k, v = inputs(n, 8, 2, 64, N, "f16")
+        o, lse = own_state(n, 8, 64, "f16")
+        lengths = torch.full((n,), N, dtype=torch.int32, device="cuda")
+        want = ck.prefix_attention(q, k, v, tail=(o, lse))
+        buf = torch.empty(n + 1, 8, 64, device="cuda", dtype=torch.float16)
+        buf[:n] = o
+        with pytest.raises(ValueError, match="overlap"):
+            ck.prefix_attention(q, k, v, tail=(buf[:n], lse), out=buf[1:])
+        assert torch.equal(ck.prefix_attention(q, k, v, tail=(buf[:n], lse), out=buf[:n]), want)
+        over = torch.empty(q.numel(), device="cuda", dtype=torch.float16)
+        state = over.view(torch.float32)[:n * 8].view(n, 8)
+        with pytest.raises(ValueError, match="overlap"):
+            ck.prefix_attention(q, k, v, tail=(o, state), out=over.view(q.shape))
+        with pytest.raises(ValueError, match="overlap"):
+            ck.prefix_attention(q, k, v, lengths=over.view(torch.int32)[:n], out=over.view(q.shape))
+        with pytest.raises(ValueError, match="overlap"):
+            odd = torch.empty(2 * q.numel(), device="cuda", dtype=torch.float16)
+            ck.prefix_attention(odd[4:4 + q.numel()].view(q.shape), k, v, out=odd[:q.numel()].view(q.shape))
+        ck.prefix_attention(q, k, v, lengths=lengths, out=buf[:n])
