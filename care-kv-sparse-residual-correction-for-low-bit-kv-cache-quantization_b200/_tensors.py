@@ -46,6 +46,36 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether tensors whose address ranges meet have no element in common for
+    this reason: they repeat with the same outer sizes and strides, and one
+    repetition of both lies within a stride with its ranges apart (slices of
+    one fused buffer)."""
+    (ap, ad), (bp, bd) = ((t.data_ptr(), sorted(((s * t.element_size(), n) for n, s in zip(t.shape, t.stride()) if n > 1),
+                                                reverse=True)) for t in (a, b))
+    ea, eb = ([t.element_size() + sum((n - 1) * s for s, n in d[i:]) for i in range(len(d) + 1)]
+              for t, d in ((a, ad), (b, bd)))
+    for i in range(min(len(ad), len(bd)) + 1):
+        if ap + ea[i] <= bp or bp + eb[i] <= ap:
+            return True
+        if i == min(len(ad), len(bd)) or ad[i] != bd[i]:
+            return False
+        if max(ap + ea[i + 1], bp + eb[i + 1]) - min(ap, bp) > ad[i][0]:
+            return False
+    return False
+
+
+def meets_itself(t: torch.Tensor) -> bool:
+    """Whether an axis steps into the elements of the axes within it (as an
+    expanded one does)."""
+    end = 1
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if s < end:
+            return True
+        end += (n - 1) * s
+    return False
+
+
 def launch(fn, t: torch.Tensor, where: str, *args):
     """fn(*args, stream) with t's device current and on its current stream;
     raises on a status other than 0.  The raw getters take 0.1 us where

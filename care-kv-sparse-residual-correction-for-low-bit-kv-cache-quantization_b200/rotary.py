@@ -17,7 +17,8 @@ import torch
 from torch import Tensor, nn
 
 from . import _lib
-from ._tensors import dtype_code, launch, need_cuda, need_like, new_rows, rows_of
+from ._tensors import (dtype_code, interleaved, launch, meets_itself, need_cuda, need_like, new_rows, overlap,
+                       rows_of)
 
 LAYOUTS = ("half", "interleaved")
 
@@ -78,7 +79,8 @@ def apply_rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, freq: Tensor
     of the inputs, which is also what autograd gets (reverse mode, any order;
     forward mode and torch.func are not supported).  out = (q_out, k_out):
     tensors of the same shapes to write to (any strides with unit channel
-    stride, apart from the inputs), new contiguous ones otherwise.
+    stride; they may lie in one buffer with each other and with the inputs, at
+    other elements), new contiguous ones otherwise.
     """
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if out is not None:
@@ -115,7 +117,7 @@ def _rows(x: Tensor, y: Tensor):
     return x.data_ptr(), y.data_ptr(), 0, t, h, 0, ot, oh, x.shape[1]
 
 
-def _check_out(q, k, out):
+def _check_out(q, k, positions, freq, out):
     yq, yk = out
     for x, y, what in ((q, yq, "q"), (k, yk, "k")):
         if (x is None) != (y is None):
@@ -125,10 +127,12 @@ def _check_out(q, k, out):
         need_like(y, q, f"apply_rotary out {what}")
         if y.shape != x.shape or (y.stride(-1) != 1 and x.shape[-1] > 1):
             raise ValueError(f"apply_rotary out {what}: expected shape {tuple(x.shape)} with unit channel stride")
-        held = y.untyped_storage().data_ptr()   # 0 without memory
-        if held and (held == q.untyped_storage().data_ptr()
-                     or (k is not None and held == k.untyped_storage().data_ptr())):
-            raise ValueError("apply_rotary out: must not share storage with q or k")
+        if y.numel() and meets_itself(y):
+            raise ValueError(f"apply_rotary out {what}: its elements overlap one another")
+        for t in (q, k, positions, freq) + ((yq,) if y is yk else ()):
+            if t is not None and overlap(y, t) and not interleaved(y, t):
+                raise ValueError("apply_rotary out: must not share storage elements with q, k, positions, freq or the "
+                                 "other result")
     return yq, yk
 
 
@@ -172,7 +176,7 @@ def _turn(q, k, positions, freq, layout, attention_factor, inverse, out):
     if k is not None:
         k = rows_of(k)
     if out is not None:
-        yq, yk = _check_out(q, k, out)
+        yq, yk = _check_out(q, k, positions, freq, out)
     else:
         yq = new_rows(q)
         yk = None if k is None else new_rows(k)

@@ -133,3 +133,39 @@ def test_prefix_object_without_a_gpu():
     sp.set(0, torch.zeros(2, 5, 8), torch.zeros(2, 5, 8))
     with pytest.raises(RuntimeError, match="CUDA"):
         sp.attend(0, torch.zeros(1, 2, 8))
+
+
+def test_overlap_of_strided_tensors():
+    """overlap / interleaved / meets_itself against the sets of elements, on views of one small buffer."""
+    import itertools
+    import random
+    pkg, _ = lib()
+    T = pkg._tensors
+    buf = torch.zeros(200, dtype=torch.float16)
+    rng = random.Random(3)
+    views = []
+    for _ in range(150):
+        shape = [rng.randint(1, 4) for _ in range(rng.randint(1, 3))]
+        stride = [rng.choice((0, 1, 2, 3, 4, 6, 8, 12, 16, 24)) for _ in shape]
+        views.append(buf.as_strided(shape, stride, rng.randint(0, 60)))
+    for base in (buf[:96].view(2, 6, 8), buf[:96].view(2, 3, 4, 4)):     # slices of fused buffers
+        for d in range(1, base.dim()):
+            for i in range(base.shape[d] + 1):
+                views += [base.narrow(d, 0, i), base.narrow(d, i, base.shape[d] - i)]
+
+    def elements(t):
+        return [t.storage_offset() + sum(i * s for i, s in zip(x, t.stride()))
+                for x in itertools.product(*(range(n) for n in t.shape))]
+    sets = [set(elements(t)) for t in views]
+    for a, sa in zip(views, sets):
+        if a.numel() and not T.meets_itself(a):
+            assert len(sa) == a.numel()
+        for b, sb in zip(views, sets):
+            if not sa.isdisjoint(sb):
+                assert T.overlap(a, b) and not T.interleaved(a, b)
+    fused = buf[:96].view(2, 6, 8)
+    for d, i in ((1, 2), (2, 3)):
+        a, b = fused.narrow(d, 0, i), fused.narrow(d, i, fused.shape[d] - i)
+        assert T.overlap(a, b) and T.interleaved(a, b) and T.interleaved(b, a)
+    assert not T.meets_itself(fused) and T.meets_itself(fused[:1].expand(3, 6, 8))
+    assert not T.overlap(buf[:10], buf[10:20]) and not T.overlap(buf[:0], buf)

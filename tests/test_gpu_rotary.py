@@ -226,3 +226,41 @@ def test_second_derivative(layout):
     check(dq.detach(), w.detach(), pos, freq, layout, 1.25, True, "f32")
     (dw,) = torch.autograd.grad((dq * u).sum(), w)
     check(dw, u, pos, freq, layout, 1.25, False, "f32")
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_results_in_one_buffer(layout):
+    """Results beside each other in one buffer (also the inputs' own, at other elements) are written in place; results
+    that meet each other, the inputs, the positions or themselves are refused."""
+    ck = pkg()
+    g = torch.Generator(device="cuda").manual_seed(8)
+    B, T, Hq, Hk, D = 2, 7, 4, 2, 64
+    freq, _ = ck.rotary_frequencies(D, device="cuda")
+    pos = torch.arange(T, device="cuda")
+    q, k = (torch.randn(B, T, h, D, device="cuda", generator=g) for h in (Hq, Hk))
+    want = ck.apply_rotary(q, k, pos, freq, layout=layout)
+
+    def same(out, q_=q, k_=k):
+        got = ck.apply_rotary(q_, k_, pos, freq, layout=layout, out=out)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    fused = torch.empty(B, T, Hq + Hk, D, device="cuda")
+    same((fused[:, :, :Hq], fused[:, :, Hq:]))
+    major = torch.empty(B, Hq + Hk, T, D, device="cuda")
+    same((major[:, :Hq].transpose(1, 2), major[:, Hq:].transpose(1, 2)))
+    wide = torch.empty(B, T, 2 * (Hq + Hk), D, device="cuda")     # inputs, then results, of every token
+    wide[:, :, :Hq], wide[:, :, Hq:Hq + Hk] = q, k
+    same((wide[:, :, Hq + Hk:2 * Hq + Hk], wide[:, :, 2 * Hq + Hk:]), wide[:, :, :Hq], wide[:, :, Hq:Hq + Hk])
+    flat = torch.empty(2, q.numel(), device="cuda")
+    flat[0] = q.flatten()
+    same((flat[1].view(q.shape), torch.empty_like(k)), flat[0].view(q.shape))
+    bad = [(fused[:, :, :Hq], fused[:, :, Hq - 1:-1]),                               # one head of both
+           (fused[:, :, :Hq], fused[:, :, :Hk]),
+           (torch.empty(B, T, 1, D, device="cuda").expand(B, T, Hq, D), torch.empty_like(k)),   # meets itself
+           (q, torch.empty_like(k)), (torch.empty_like(q), k),
+           (torch.empty_like(q), q[:, :, :Hk])]
+    for out in bad:
+        with pytest.raises(ValueError, match="overlap|share storage"):
+            ck.apply_rotary(q, k, pos, freq, layout=layout, out=out)
+    room = torch.zeros(q.numel(), device="cuda")
+    with pytest.raises(ValueError, match="overlap|share storage"):
+        ck.apply_rotary(q, k, room.view(torch.int64)[:T], freq, layout=layout, out=(room.view(q.shape), torch.empty_like(k)))
