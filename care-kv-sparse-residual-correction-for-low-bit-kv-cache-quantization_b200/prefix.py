@@ -113,13 +113,16 @@ class SharedPrefix:
         self._kv = [None] * num_layers
 
     def set(self, layer: int, k: Tensor, v: Tensor):
-        """k, v [Hkv, N, D] of one layer."""
+        """k, v [Hkv, N, D] of one layer (copied).  A layer may be set anew; all
+        layers hold the same number of tokens."""
         if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
             raise ValueError(f"SharedPrefix: k {tuple(k.shape)} and v {tuple(v.shape)} must match")
-        n = self.tokens
+        self._kv[layer]   # an index that there is
+        n = next((kv[0].shape[1] for i, kv in enumerate(self._kv)
+                  if kv is not None and i != layer % len(self._kv)), None)
         if n is not None and k.shape[1] != n:
             raise ValueError(f"SharedPrefix: layer {layer} holds {k.shape[1]} tokens, the others {n}")
-        self._kv[layer] = (k.contiguous(), v.contiguous())
+        self._kv[layer] = tuple(t.detach().clone(memory_format=torch.contiguous_format) for t in (k, v))
 
     @property
     def tokens(self) -> Optional[int]:

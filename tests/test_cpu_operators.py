@@ -169,3 +169,18 @@ def test_overlap_of_strided_tensors():
         assert T.overlap(a, b) and T.interleaved(a, b) and T.interleaved(b, a)
     assert not T.meets_itself(fused) and T.meets_itself(fused[:1].expand(3, 6, 8))
     assert not T.overlap(buf[:10], buf[10:20]) and not T.overlap(buf[:0], buf)
+
+
+def test_prefix_layers_set_anew():
+    pkg, _ = lib()
+    sp = pkg.SharedPrefix(2)
+    k = torch.ones(2, 5, 8)
+    sp.set(1, k, k)
+    sp.set(-1, k[:, :3], k[:, :3])          # the same layer, alone so far: another length
+    assert sp.tokens == 3 and sp.layer(1)[0].is_contiguous()
+    k.zero_()
+    assert bool((sp.layer(1)[0] == 1).all())
+    with pytest.raises(ValueError, match="the others 3"):
+        sp.set(0, k, k)
+    with pytest.raises(IndexError):
+        sp.set(2, k[:, :3], k[:, :3])

@@ -391,3 +391,21 @@ def test_result_over_the_own_state():
             odd = torch.empty(2 * q.numel(), device="cuda", dtype=torch.float16)
             ck.prefix_attention(odd[4:4 + q.numel()].view(q.shape), k, v, out=odd[:q.numel()].view(q.shape))
         ck.prefix_attention(q, k, v, lengths=lengths, out=buf[:n])
+
+
+def test_shared_prefix_holds_its_own_values():
+    """A later write to the tensors given to set() does not change the prefix; a layer can be set anew, to another
+    length too where no other layer holds one."""
+    ck = pkg()
+    q, k, v = inputs(4, 8, 2, 64, 100, "f16")
+    sp = ck.SharedPrefix(1)
+    sp.set(0, k, v)
+    want = sp.attend(0, q)
+    k.zero_()
+    v.zero_()
+    assert torch.equal(sp.attend(0, q), want)
+    _, k, v = inputs(4, 8, 2, 64, 60, "f16", 3)
+    sp.set(0, k, v)
+    assert sp.tokens == 60 and torch.equal(sp.attend(0, q), ck.prefix_attention(q, k, v))
+    sp.set(0, k.float().requires_grad_(), v.float())
+    assert not sp.layer(0)[0].requires_grad
