@@ -159,8 +159,8 @@ class DecodeEngine:
         CAREKV_DECODE_ROUTER.
         prefix: tokens shared by all sequences, before their own: the cache's
         result (its residual correction routed over the own tokens alone) is
-        merged with attention over the prefix of this layer (same dtype and
-        kv heads as the cache's).
+        merged with attention over the prefix of this layer (dtype of q, kv
+        heads and head size of this arena).
         return_lse: also the fp32 log-sum-exp [seq_count, Hq] of the attention.
         The results carry no graph."""
         cfg = self.cfg
@@ -174,6 +174,8 @@ class DecodeEngine:
                                   k_corr_scale=k_corr_scale, legacy=decode_router(router) == "cached")
         if not correction:
             rp.kind = _lib.KIND_NONE
+        if prefix is not None:
+            prefix.check(layer, cfg.num_kv_heads, cfg.head_dim, q.dtype)
         nbytes = self.workspace_bytes(n, pages)
         ws = self.workspace(nbytes)
         lse = None

@@ -208,8 +208,10 @@ class CAREKVLayer(nn.Module):
         B, T, _ = hidden.shape
         g = cfg.num_heads // cfg.num_kv_heads
         q, k, v = self._project(hidden)
-        if prefix is not None and torch.is_grad_enabled() and (q.requires_grad or v.requires_grad):
-            raise RuntimeError("prefill with a prefix has no backward pass: call it under no_grad")
+        if prefix is not None:
+            prefix.check(self.layer_id, cfg.num_kv_heads, cfg.head_dim, q.dtype)
+            if torch.is_grad_enabled() and (q.requires_grad or v.requires_grad):
+                raise RuntimeError("prefill with a prefix has no backward pass: call it under no_grad")
         q_post, k_post = self._rotate(q, k, position_embeddings, positions)
         eng = engine_for(cache)
         eng.prefill_store(self.layer_id, k_post.contiguous(), v.contiguous(), seq_begin=seq_begin,
@@ -349,6 +351,8 @@ class CAREKVLayer(nn.Module):
             if cos.shape[0] == 1 and B > 1:
                 cos, sin = cos.expand(B, 1, -1), sin.expand(B, 1, -1)
             pe = (cos, sin)
+        if prefix is not None:   # before the token enters the cache
+            prefix.check(self.layer_id, cfg.num_kv_heads, cfg.head_dim, q.dtype)
         q_post, k_post = self._rotate(q, k, pe, None if positions is None else positions.reshape(B, 1))
         eng = engine_for(cache)
         eng.append(self.layer_id, k_post[:, :, 0].contiguous(), v[:, :, 0].contiguous(), seq_begin=seq_begin)

@@ -135,6 +135,13 @@ class SharedPrefix:
             raise ValueError(f"SharedPrefix: layer {layer} has not been set")
         return kv
 
+    def check(self, layer: int, kv_heads: int, head_dim: int, dtype: torch.dtype):
+        """Raises unless the layer is set, to that many kv heads of that size and dtype."""
+        k, _ = self.layer(layer)
+        if k.dtype != dtype or k.shape[0] != kv_heads or k.shape[2] != head_dim:
+            raise ValueError(f"SharedPrefix: expected {dtype} [{kv_heads}, tokens, {head_dim}] as the cache's kv heads, "
+                             f"got {k.dtype} {tuple(k.shape)}")
+
     def memory_bytes(self) -> int:
         return sum(2 * kv[0].numel() * kv[0].element_size() for kv in self._kv if kv is not None)
 

@@ -347,3 +347,41 @@ def test_quantized_layer_is_copied_saved_and_moved(pkg):
     assert all(getattr(odd, n) is not None for n in ("W_Q", "W_K", "W_V", "W_O"))
     dense = make()
     assert set(dense.state_dict()) == {"W_Q", "W_K", "W_V", "W_O"}
+
+
+def test_prefix_that_does_not_fit_the_cache_is_refused(pkg):
+    """A prefix of other kv heads, head size or type than the arena's is an error before anything is written."""
+    with env(**PAPER_BEST_ENV):
+        cfg, cache, eng, seqs, q = build(pkg, 64, 3, 32, 8, 4, "fp16", (20, 5), 3, read_budget_mode="absolute",
+                                         read_abs_k=1, read_abs_v=1)
+        qt = torch.from_numpy(q).cuda().half()
+        out = torch.full_like(qt, 7.0)
+
+        def prefix(h, d, dt):
+            sp = pkg.SharedPrefix(1)
+            sp.set(0, torch.randn(h, 50, d, device="cuda").to(dt), torch.randn(h, 50, d, device="cuda").to(dt))
+            return sp
+        for sp in (prefix(2, 64, torch.float16), prefix(8, 64, torch.float16), prefix(4, 128, torch.float16),
+                   prefix(4, 64, torch.bfloat16), pkg.SharedPrefix(1)):
+            with pytest.raises(ValueError, match="prefix|SharedPrefix"):
+                eng.attend(0, qt, out=out, prefix=sp)
+        assert bool((out == 7.0).all())
+        eng.attend(0, qt, out=out, prefix=prefix(4, 64, torch.float16))
+
+
+def test_layer_calls_refuse_a_prefix_before_the_cache_is_written(pkg):
+    with env(CAREKV_PREFILL_MODE="fp", **PAPER_BEST_ENV):
+        cfg = pkg.CacheConfig(num_layers=1, num_heads=4, num_kv_heads=4, head_dim=64, max_pages=4, base_bits=3,
+                              group_size=32, scale_quant="int8", store_budget_mode="absolute", store_abs_k=1,
+                              store_abs_v=1, read_budget_mode="absolute", read_abs_k=1, read_abs_v=1)
+        W = torch.randn(256, 64, device="cuda")
+        layer = pkg.CAREKVLayer(cfg, 0, W, W, W, W.T.contiguous(), torch.device("cuda"))
+        cache = pkg.CAREKVCache(cfg, torch.device("cuda"), batch=1)
+        sp = pkg.SharedPrefix(1)
+        sp.set(0, torch.randn(2, 20, 64, device="cuda"), torch.randn(2, 20, 64, device="cuda"))
+        hid = torch.randn(1, 5, 64, device="cuda")
+        with pytest.raises(ValueError, match="SharedPrefix"):
+            layer.prefill_batch(cache, hid, prefix=sp)
+        with pytest.raises(ValueError, match="SharedPrefix"):
+            layer.decode_step_batch(cache, hid[:, 0], prefix=sp)
+        assert cache.total_valid_tokens(0, 0) == 0
