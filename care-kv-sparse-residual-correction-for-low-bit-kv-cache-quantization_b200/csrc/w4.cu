@@ -194,7 +194,8 @@ struct Act<CAREKV_F32> {
   using S = float;
   // x = hi + mid + lo: each term the upper 16 bits of what is left, 8
   // significand bits of the 24, so the split is exact (down to bf16's
-  // smallest numbers); infinities and NaN stay in the first term
+  // smallest numbers); infinities and NaN stay in the first term, a NaN by its
+  // quiet bit (its payload may lie in the lower 16 bits alone)
   static __device__ __forceinline__ void load(const T* p, uint32_t (&b)[3][4]) {
     float x[8];
     *reinterpret_cast<float4*>(x) = __ldg(reinterpret_cast<const float4*>(p));
@@ -203,7 +204,11 @@ struct Act<CAREKV_F32> {
     for (int i = 0; i < 3; ++i) {
 #pragma unroll
       for (int k = 0; k < 8; k += 2) {
-        const uint32_t lo = __float_as_uint(x[k]), hi = __float_as_uint(x[k + 1]);
+        uint32_t lo = __float_as_uint(x[k]), hi = __float_as_uint(x[k + 1]);
+        if (i == 0) {
+          if ((lo & 0x7fffffffu) > 0x7f800000u) lo |= 0x00400000u;
+          if ((hi & 0x7fffffffu) > 0x7f800000u) hi |= 0x00400000u;
+        }
         b[i][k / 2] = prmt(lo, hi, 0x7632);
         x[k] = (lo & 0x7f800000u) == 0x7f800000u ? 0.f : x[k] - __uint_as_float(lo & 0xffff0000u);
         x[k + 1] = (hi & 0x7f800000u) == 0x7f800000u ? 0.f : x[k + 1] - __uint_as_float(hi & 0xffff0000u);

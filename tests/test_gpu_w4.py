@@ -249,3 +249,48 @@ def test_copies_and_checkpoints():
         away.dequantize()
     assert torch.equal(away.cuda().matvec(x), want)
     assert torch.equal(copy.deepcopy(pw).bfloat16().matvec(x), want)      # codes and scales are bytes: no cast
+
+
+def test_every_nan_of_fp32_stays_one():
+    """fp32 NaN whose payload lies in the low half only; infinities stay infinities."""
+    ck = pkg()
+    packed, scale, w = weight(24, 64, 32, "f32", 42)
+    x = torch.randn(4, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    bits = x.view(torch.int32)
+    bits[1, 9], bits[2, 9] = 0x7F800001, -(1 << 23) + 1      # 0xFF800001
+    y = ck.PackedWeight(packed, scale, 32).matvec(x)
+    assert bool(y[1].isnan().all()) and bool(y[2].isnan().all())
+    check(y[0::3], x[0::3], w, "f32")
+
+
+@pytest.mark.parametrize("k,group", [(64, 32), (256, 128), (160, 32)])
+def test_low_bits_of_fp32_activations(k, group):
+    """Activations 1 and 1 + e 2^-23 under codes c and -c: what is left is c e 2^-23, held in the lowest of the three
+    terms of an activation alone.  The codes' products of the upper terms cancel exactly (small integers, adjacent
+    channels in one product), so the bound is that of the fp32 sum of what is left."""
+    ck = pkg()
+    g = torch.Generator(device="cuda").manual_seed(k)
+    n, m = 40, 9
+    codes = torch.randint(-7, 8, (n, k // 2, 1), device="cuda", generator=g) * torch.tensor([1, -1], device="cuda")
+    codes = codes.view(n, k)
+    packed = ((codes[:, 0::2] & 15) | ((codes[:, 1::2] & 15) << 4)).to(torch.uint8)
+    scale = 0.5 + torch.rand(n, k // group, device="cuda", generator=g)
+    e = torch.randint(0, 128, (m, k // 2), device="cuda", generator=g)
+    x = torch.ones(m, k, device="cuda")
+    x[:, 0::2] += e * 2.0 ** -23
+    w = codes.double() * scale.double().repeat_interleave(group, 1)
+    ref = x.double() @ w.T
+    size = (x.double() - 1) @ w.abs().T
+    err = (ck.PackedWeight(packed, scale, group).matvec(x).double() - ref).abs()
+    assert bool((err <= k * 2.0 ** -24 * size).all()), float((err / size).max())
+
+
+def test_one_row_of_any_stride():
+    """A single row's distance to the next is never used: cut from rows of odd length it is one row like any other."""
+    ck = pkg()
+    for dtype in DT:
+        packed, scale, w = weight(20, 64, 32, dtype, 40)
+        pw = ck.PackedWeight(packed, scale, 32)
+        wide = torch.randn(4, 67, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(DT[dtype])
+        for x in (wide[:1, :64], wide[1:2, 3:], wide[None, 2:3, 1:65], wide.t()[:64].t()[3:]):
+            check(pw.matvec(x), x, w, dtype)
