@@ -759,10 +759,20 @@ cudaError_t launch_w4_dequant(const carekv_w4_t& w, void* out, cudaStream_t st) 
 }
 
 cudaError_t launch_w4(const carekv_w4_t& w, const void* x, int64_t ldx, int M, void* out, cudaStream_t st) {
-  if (M == 0) return cudaSuccess;
-  if (w.dtype == CAREKV_F16) return launch_dt<CAREKV_F16>(w, x, ldx, M, out, st);
-  if (w.dtype == CAREKV_BF16) return launch_dt<CAREKV_BF16>(w, x, ldx, M, out, st);
-  return launch_dt<CAREKV_F32>(w, x, ldx, M, out, st);
+  // rows lie along grid.y, 8 at least to a CTA: 65535 of them in one launch
+  constexpr int kMost = 8 * 65535;
+  const int es = w.dtype == CAREKV_F32 ? 4 : 2;
+  for (int m = 0; m < M;) {
+    const int n = std::min(M - m, kMost);
+    const void* xm = static_cast<const char*>(x) + m * ldx * es;
+    void* om = static_cast<char*>(out) + static_cast<int64_t>(m) * w.n * es;
+    const cudaError_t e = w.dtype == CAREKV_F16    ? launch_dt<CAREKV_F16>(w, xm, ldx, n, om, st)
+                          : w.dtype == CAREKV_BF16 ? launch_dt<CAREKV_BF16>(w, xm, ldx, n, om, st)
+                                                   : launch_dt<CAREKV_F32>(w, xm, ldx, n, om, st);
+    if (e != cudaSuccess) return e;
+    m += n;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace carekv

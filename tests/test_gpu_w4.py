@@ -294,3 +294,11 @@ def test_one_row_of_any_stride():
         wide = torch.randn(4, 67, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(DT[dtype])
         for x in (wide[:1, :64], wide[1:2, 3:], wide[None, 2:3, 1:65], wide.t()[:64].t()[3:]):
             check(pw.matvec(x), x, w, dtype)
+
+
+@pytest.mark.parametrize("dtype,rows", [("f32", 8 * 65535 + 21), ("f16", 16 * 65535 + 37)])
+def test_more_rows_than_one_launch_takes(dtype, rows):
+    ck = pkg()
+    packed, scale, w = weight(5, 32, 32, dtype, 41)
+    x = torch.randn(rows, 32, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(DT[dtype])
+    check(ck.PackedWeight(packed, scale, 32).matvec(x), x, w, dtype)
