@@ -626,12 +626,16 @@ cudaError_t launch_few(const carekv_w4_t& w, const void* x, int64_t ldx, int M, 
                                                           panels, kKeys<A::kF16>, static_cast<typename A::T*>(out));
   return cudaGetLastError();
 }
-// Clusters of 1 .. 8 CTAs of `kernel` that the device holds at once.
+// Clusters of `size` (1 .. 8) CTAs of `kernel` that the current device holds at
+// once; asked once per host thread, device and kernel.
 template <typename K>
 int max_clusters(K* kernel, int size, int threads, int smem) {
-  static thread_local const void* known[9] = {};
-  static thread_local int count[9] = {};
-  if (known[size] == reinterpret_cast<const void*>(kernel)) return count[size];
+  static thread_local const void* known[64][9] = {};
+  static thread_local int count[64][9] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  const bool keep = dev >= 0 && dev < 64;
+  if (keep && known[dev][size] == reinterpret_cast<const void*>(kernel)) return count[dev][size];
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(size);
   cfg.blockDim = dim3(threads);
@@ -646,8 +650,10 @@ int max_clusters(K* kernel, int size, int threads, int smem) {
     (void)cudaGetLastError();
     return 0;
   }
-  known[size] = reinterpret_cast<const void*>(kernel);
-  count[size] = n;
+  if (keep) {
+    known[dev][size] = reinterpret_cast<const void*>(kernel);
+    count[dev][size] = n;
+  }
   return n;
 }
 
