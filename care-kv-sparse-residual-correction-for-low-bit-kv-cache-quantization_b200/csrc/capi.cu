@@ -418,6 +418,10 @@ int carekv_decode_attention_launches(const carekv_config_t* cfg, int32_t seq_cou
   return CAREKV_OK;
 }
 
+// Most rows, heads or channels of one call: a tile's worth above them still
+// fits the kernels' 32-bit row counters.
+static constexpr int64_t kMostRows = INT32_MAX - 4096;
+
 int carekv_rotary(const carekv_rotary_t* a, void* stream) {
   if (!a || !a->freq || a->batch < 0 || a->tokens < 0 || a->q.heads < 0 || a->k.heads < 0) return CAREKV_ERR_INVALID_ARG;
   if (a->head_dim < 1 || a->rotary_dim < 2 || a->rotary_dim % 2 || a->rotary_dim > a->head_dim)
@@ -426,8 +430,8 @@ int carekv_rotary(const carekv_rotary_t* a, void* stream) {
   if (a->position_bytes != 4 && a->position_bytes != 8) return CAREKV_ERR_INVALID_ARG;
   CHECK(validate_dtype(a->dtype));
   const int64_t tok = static_cast<int64_t>(a->batch) * a->tokens;
-  if (tok > INT32_MAX || tok * (static_cast<int64_t>(a->q.heads) + a->k.heads) > (int64_t{1} << 40))
-    return CAREKV_ERR_UNSUPPORTED;
+  const int64_t heads = static_cast<int64_t>(a->q.heads) + a->k.heads;
+  if (tok > kMostRows || heads > kMostRows || tok * heads > (int64_t{1} << 40)) return CAREKV_ERR_UNSUPPORTED;
   if (tok == 0) return CAREKV_OK;
   if (!a->positions) return CAREKV_ERR_INVALID_ARG;
   for (const carekv_rows_t* r : {&a->q, &a->k})
@@ -438,6 +442,7 @@ int carekv_rotary(const carekv_rotary_t* a, void* stream) {
 static int validate_w4(const carekv_w4_t* w) {
   if (!w || w->n < 1 || w->k < 1 || w->group_size < 1 || w->k % w->group_size) return CAREKV_ERR_INVALID_ARG;
   if (w->group_size != 32 && w->group_size != 64 && w->group_size % 128) return CAREKV_ERR_UNSUPPORTED;
+  if (w->n > kMostRows || w->k > kMostRows) return CAREKV_ERR_UNSUPPORTED;
   return validate_dtype(w->dtype);
 }
 static int validate_w4_buffers(const carekv_w4_t* w) {
@@ -478,7 +483,7 @@ int carekv_w4_matvec(const carekv_w4_t* w, const void* x, int64_t x_stride, int3
 static int validate_prefix(const carekv_prefix_t* p, int32_t rows, int32_t heads) {
   if (!p || p->num_kv_heads < 1 || p->tokens < 0 || p->head_dim < 1 || rows < 0 || heads < 1) return CAREKV_ERR_INVALID_ARG;
   if (heads % p->num_kv_heads) return CAREKV_ERR_INVALID_ARG;
-  if (p->head_dim > 256 || p->num_kv_heads > 65535 || p->tokens > (1 << 30) || static_cast<int64_t>(rows) * heads > INT32_MAX)
+  if (p->head_dim > 256 || p->num_kv_heads > 65535 || p->tokens > (1 << 30) || static_cast<int64_t>(rows) * heads > kMostRows)
     return CAREKV_ERR_UNSUPPORTED;
   return validate_dtype(p->dtype);
 }

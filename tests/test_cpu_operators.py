@@ -184,3 +184,24 @@ def test_prefix_layers_set_anew():
         sp.set(0, k, k)
     with pytest.raises(IndexError):
         sp.set(2, k[:, :3], k[:, :3])
+
+
+def test_sizes_beyond_the_row_counters():
+    """Sizes whose last tile would pass a 32-bit row counter are refused before any launch."""
+    pkg, l = lib()
+    most = 2 ** 31 - 1
+
+    def rotary(tokens, heads):
+        rows = (16, 32, 0, 1, 1, 0, 1, 1)
+        return l.carekv_rotary(pkg._lib.ROTARY_PACK(*rows, heads, *rows, 1, 16, 16, 0, 1, 8, 1, tokens, 2, 2, 0, 0, 1.0,
+                                                    1), None)
+    assert rotary(most, 1) == 2 and rotary(most - 1000, 1) == 2
+    assert rotary(1, most) == 2 and rotary(1, most - 1) == 2
+    w, sizes = pkg._lib.W4(), (ctypes.c_size_t * 2)()
+    for n, k in ((most, 32), (most - 1000, 32), (1, 2 ** 31 - 128)):
+        w.n, w.k, w.group_size, w.dtype = n, k, 32, 1
+        assert l.carekv_w4_layout(ctypes.byref(w), sizes) == 2
+    need = ctypes.c_size_t(0)
+    for rows, heads in ((most, 1), (1 << 30, 2), (most - 1000, 1)):
+        assert l.carekv_prefix_workspace_bytes(pkg._lib.PREFIX_PACK(0, 0, 0, 0, 0, 0, 1, 100, 64, 1), rows, heads,
+                                               ctypes.byref(need)) == 2
