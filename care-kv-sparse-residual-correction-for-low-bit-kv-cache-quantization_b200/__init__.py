@@ -16,6 +16,7 @@ from .quantizer import (QuantConfig, KQuantizer, VQuantizer, quantize, dequantiz
 from .rotary import RotaryEmbedding, apply_rotary, rotary_frequencies
 from .weights import PackedWeight
 from .prefix import SharedPrefix, prefix_attention
+from ._tensors import check_operator_errors
 from .engine import DecodeEngine
 from .layer import CAREKVLayer, causal_attention, resolve_prefill_mode
 from .llama_patch import CAREKVLlamaAttention, patch_llama_model, reset_all_caches
@@ -31,6 +32,7 @@ __all__ = [
     "pack_codes_2d", "unpack_codes_2d", "packed_row_bytes", "pack_4bit", "unpack_4bit",
     "quant_dequant_kivi_k", "quant_dequant_kivi_v",
     "RotaryEmbedding", "apply_rotary", "rotary_frequencies", "PackedWeight", "SharedPrefix", "prefix_attention",
+    "check_operator_errors",
     "DecodeEngine", "CAREKVLayer", "causal_attention", "resolve_prefill_mode",
     "CAREKVLlamaAttention", "patch_llama_model", "reset_all_caches", "CAREKVAdapter",
 ]

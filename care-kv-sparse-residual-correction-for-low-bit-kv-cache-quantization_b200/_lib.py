@@ -137,6 +137,7 @@ SIGNATURES = [
     ("carekv_decode_attention_lse", i32, [ctypes.POINTER(Config), ctypes.POINTER(Cache), i32, vp, vp, vp, i32, i32,
                                           i32, i32, ctypes.POINTER(RouteParams), vp, vp, ctypes.c_size_t,
                                           ctypes.POINTER(Shard), vp]),
+    ("carekv_check_operator_errors", i32, [ctypes.POINTER(i32), vp]),
     ("carekv_rotary", i32, [vp, vp]),   # carekv_rotary_t as packed bytes
     ("carekv_w4_layout", i32, [ctypes.POINTER(W4), ctypes.POINTER(ctypes.c_size_t)]),
     ("carekv_w4_pack", i32, [ctypes.POINTER(W4), vp, vp, vp]),

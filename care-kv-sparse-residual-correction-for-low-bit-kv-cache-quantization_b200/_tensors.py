@@ -89,3 +89,12 @@ def launch(fn, t: torch.Tensor, where: str, *args):
             status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status, where)
+
+
+def check_operator_errors(device=None):
+    """Raises if a wait inside a 4-bit product or a shared-prefix attention on
+    the device (default: the current one) ran out since the last check; such a
+    call's rows are NaN.  Synchronizes the device's current stream."""
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().carekv_check_operator_errors(None, torch.cuda.current_stream().cuda_stream),
+                   "operator check")

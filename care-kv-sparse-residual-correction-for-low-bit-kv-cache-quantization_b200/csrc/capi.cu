@@ -510,6 +510,14 @@ int carekv_prefix_attention(const carekv_prefix_t* p, const void* q, int64_t q_r
                                    out, lse, ws, as_stream(stream)));
 }
 
+int carekv_check_operator_errors(int32_t* flags_out, void* stream) {
+  int32_t w4 = 0, prefix = 0;
+  CHECK(cuda_status(w4_wait_errors(&w4, as_stream(stream))));
+  CHECK(cuda_status(prefix_wait_errors(&prefix, as_stream(stream))));
+  if (flags_out) *flags_out = (w4 ? 1 : 0) | (prefix ? 2 : 0);
+  return w4 || prefix ? CAREKV_ERR_DEVICE_CHECK : CAREKV_OK;
+}
+
 int carekv_check_device_errors(const carekv_cache_t* cache, int32_t* flags_out, void* stream) {
   if (!cache || !cache->error_flag) return CAREKV_ERR_INVALID_ARG;
   int32_t h = 0;

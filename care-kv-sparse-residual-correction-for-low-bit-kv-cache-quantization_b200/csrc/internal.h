@@ -41,6 +41,8 @@ size_t prefix_workspace_bytes(const carekv_prefix_t& p, int rows, int heads);
 cudaError_t launch_prefix(const carekv_prefix_t& p, const void* q, int64_t q_row, int64_t q_head, int rows, int heads,
                           float scale, const int32_t* lengths, const void* tail, const float* tail_lse, void* out,
                           float* lse, void* ws, cudaStream_t st);
+cudaError_t w4_wait_errors(int32_t* set, cudaStream_t st);      // a wait of these kernels ran out: read and cleared
+cudaError_t prefix_wait_errors(int32_t* set, cudaStream_t st);
 struct DecodeArgs;
 template <int QN>
 cudaError_t launch_decode_generic(DecodeArgs& a, cudaStream_t st, int n_bh);

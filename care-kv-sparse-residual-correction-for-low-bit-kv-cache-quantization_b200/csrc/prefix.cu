@@ -736,6 +736,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
   }
   tc_fence_before();
   __syncthreads();
+  report_wait(dead);
   if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(*tmem_slot, 512);
@@ -985,6 +986,8 @@ cudaError_t launch_combine(const PrefixArgs& a, cudaStream_t st) {
 }
 
 }  // namespace
+
+cudaError_t prefix_wait_errors(int32_t* set, cudaStream_t st) { return take_wait_errors(set, st); }
 
 // room for either form, and for the partial sums to start on a 32-byte
 // boundary (store32) in a buffer that starts on one of 16

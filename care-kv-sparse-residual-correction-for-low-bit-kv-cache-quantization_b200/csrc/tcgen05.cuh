@@ -2,6 +2,7 @@
 // allocation and access, descriptors, tcgen05.mma, and tiled TMA loads.
 #pragma once
 #include <cuda.h>
+#include <cuda_runtime.h>
 #include <cstdint>
 
 #include "ptx.cuh"
@@ -148,6 +149,21 @@ __device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile
     }
   }
   return true;
+}
+// Set by a CTA one of whose waits gave up; its results are NaN.  One per
+// source file; the host takes it with take_wait_errors.
+static __device__ int wait_errors;
+__device__ __forceinline__ void report_wait(volatile int* dead) {   // once per CTA, after its last barrier
+  if (threadIdx.x == 0 && *dead) atomicOr(&wait_errors, 1);
+}
+// Reads and clears the flag (synchronizes the stream).
+static inline cudaError_t take_wait_errors(int32_t* set, cudaStream_t st) {
+  void* p = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&p, wait_errors);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(set, p, sizeof(int), cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && *set) e = cudaMemsetAsync(p, 0, sizeof(int), st);
+  return e;
 }
 // two fp32 operations per instruction
 __device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {

@@ -566,7 +566,10 @@ __global__ void __launch_bounds__(TcLayout<NS, NT>::kThreads, 1)
     }
     if (issuer) {   // nothing of ours may still run or arrive when the CTA ends
       mma_commit(done, lead);
-      mbar_wait(done, 0);
+      if (!mbar_wait(done, 0)) {
+        *dead = 1;
+        ok = false;
+      }
     }
     __syncwarp();
     if (!ok) {   // a wait ran out: the rows say so
@@ -609,6 +612,7 @@ __global__ void __launch_bounds__(TcLayout<NS, NT>::kThreads, 1)
   } else {
     __syncthreads();
   }
+  report_wait(dead);
   if (warp == kLoad) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -740,6 +744,8 @@ int64_t tiles(int n, int k) {
 }
 
 }  // namespace
+
+cudaError_t w4_wait_errors(int32_t* set, cudaStream_t st) { return take_wait_errors(set, st); }
 
 void w4_layout(int n, int k, int group, int dt, size_t sizes[2]) {
   const int64_t t = tiles(n, k);

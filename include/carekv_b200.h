@@ -508,6 +508,13 @@ int carekv_prefix_attention(const carekv_prefix_t *prefix, const void *q, int64_
                             const int32_t *lengths, const void *tail_out, const float *tail_lse, void *out,
                             float *lse, void *workspace, size_t workspace_bytes, void *stream);
 
+/* Whether a wait inside carekv_w4_matvec (bit 0 of flags_out, which may be
+ * NULL) or carekv_prefix_attention (bit 1) ran out on the current device since
+ * the last call: about a second without progress, after which the kernel gives
+ * up and its rows are NaN.  Synchronizes the stream and clears the flags;
+ * CAREKV_ERR_DEVICE_CHECK when one was set. */
+int carekv_check_operator_errors(int32_t *flags_out, void *stream);
+
 /* Copy the device error flag to the host and clear it (synchronizes the
  * stream).  Returns CAREKV_OK when no device check tripped. */
 int carekv_check_device_errors(const carekv_cache_t *cache, int32_t *flags_out, void *stream);
