@@ -877,7 +877,7 @@ __global__ void __launch_bounds__(256) prefix_fma_combine_kernel(const PrefixArg
 int fma_splits(const carekv_prefix_t& p, int rows, int heads) {
   const int64_t ctas = static_cast<int64_t>(p.num_kv_heads) *
                        ((static_cast<int64_t>(rows) * (heads / p.num_kv_heads) + kFmaRows - 1) / kFmaRows);
-  const int want = static_cast<int>(std::min<int64_t>(64, (2 * 148 + ctas - 1) / std::max<int64_t>(1, ctas)));
+  const int want = static_cast<int>(std::min<int64_t>(64, (2 * sm_count() + ctas - 1) / std::max<int64_t>(1, ctas)));
   return std::max(1, std::min(want, (p.tokens + 127) / 128));
 }
 

@@ -714,18 +714,18 @@ cudaError_t launch_tc(const carekv_w4_t& w, const void* x, int64_t ldx, int M, v
 // 2.7 against 9.5.
 template <int DT, int NS>
 cudaError_t launch_ns(const carekv_w4_t& w, const void* x, int64_t ldx, int M, void* out, cudaStream_t st) {
-  const int panels = (w.n + kTileRows - 1) / kTileRows;
+  const int panels = (w.n + kTileRows - 1) / kTileRows, sms = sm_count();
   if (M <= 8 || DT == CAREKV_F32) {
-    if (panels >= 4 * 148) return launch_few<DT, NS, 1, 1, 4>(w, x, ldx, M, out, st);
-    if (panels >= 2 * 148) return launch_few<DT, NS, 1, 1, 8>(w, x, ldx, M, out, st);
+    if (panels >= 4 * sms) return launch_few<DT, NS, 1, 1, 4>(w, x, ldx, M, out, st);
+    if (panels >= 2 * sms) return launch_few<DT, NS, 1, 1, 8>(w, x, ldx, M, out, st);
     return launch_few<DT, NS, 1, 1, 16>(w, x, ldx, M, out, st);
   }
   if constexpr (DT != CAREKV_F32) {
     const int64_t codes = static_cast<int64_t>(w.n) * w.k;
     if (M > 32 && codes >= (8 << 20)) return launch_tc<DT, NS, 64>(w, x, ldx, M, out, st);
     if (M > 16 && M <= 32 && codes >= (32 << 20)) return launch_tc<DT, NS, 32>(w, x, ldx, M, out, st);
-    if (panels >= (M > 16 ? 148 : 4 * 148)) return launch_few<DT, NS, 2, 2, 4>(w, x, ldx, M, out, st);
-    if (panels >= 148) return launch_few<DT, NS, 2, 1, 8>(w, x, ldx, M, out, st);
+    if (panels >= (M > 16 ? sms : 4 * sms)) return launch_few<DT, NS, 2, 2, 4>(w, x, ldx, M, out, st);
+    if (panels >= sms) return launch_few<DT, NS, 2, 1, 8>(w, x, ldx, M, out, st);
     return launch_few<DT, NS, 2, 1, 16>(w, x, ldx, M, out, st);
   }
   return cudaErrorInvalidValue;
