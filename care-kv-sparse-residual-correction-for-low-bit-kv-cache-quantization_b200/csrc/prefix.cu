@@ -161,9 +161,10 @@ constexpr int kTcThreads = 320, kTcRows = 128, kTcBlock = 128;
 constexpr float kRaise = 8.f;
 // One of so many pairs of weights is computed on the FMA pipe: the 16
 // special-function lanes of an SM take 2048 cycles for a block's 256 rows x
-// 128 weights, half of what the block takes (512 rows x 8 heads of 64 on 8192
-// tokens: 86 us without, 81 with every fourth, 84 with three of eight).
-constexpr int kFmaEvery = 4;
+// 128 weights, half of what the block takes (2048 rows x 32 heads of 128 on
+// 8192 tokens of 8 kv heads, calls back to back: 288 us without, 278 with
+// every eighth, 284 with every fourth, 299 with every second).
+constexpr int kFmaEvery = 8;
 
 template <int D, bool PAIR>
 struct TcLayout {
