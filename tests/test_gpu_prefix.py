@@ -409,3 +409,34 @@ def test_shared_prefix_holds_its_own_values():
     assert sp.tokens == 60 and torch.equal(sp.attend(0, q), ck.prefix_attention(q, k, v))
     sp.set(0, k.float().requires_grad_(), v.float())
     assert not sp.layer(0)[0].requires_grad
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_many_rows_on_a_long_prefix(dtype):
+    ck = pkg()
+    for n, hq, hkv, D, N in ((300, 4, 2, 128, 5003), (260, 2, 2, 64, 9000)):
+        q, k, v = inputs(n, hq, hkv, D, N, dtype, n)
+        o, lse = ck.prefix_attention(q, k, v, return_lse=True)
+        check(o, lse, q, k, v, dtype)
+
+
+def test_results_repeat_and_run_in_a_graph():
+    """The same bits at every call, and from a captured graph (also with other values in the same tensors)."""
+    ck = pkg()
+    for n, hq, hkv, D, N in ((2, 8, 2, 64, 300), (20, 8, 8, 128, 3000), (300, 4, 2, 128, 3000)):
+        q, k, v = inputs(n, hq, hkv, D, N, "bf16", 5)
+        tail = own_state(n, hq, D, "bf16")
+        want = ck.prefix_attention(q, k, v, tail=tail, return_lse=True)
+        for _ in range(20):
+            got = ck.prefix_attention(q, k, v, tail=tail, return_lse=True)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o, lse = ck.prefix_attention(q, k, v, tail=tail, return_lse=True)
+        graph.replay()
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+        q.neg_()
+        graph.replay()
+        assert not torch.equal(o, want[0])
+        got = ck.prefix_attention(q, k, v, tail=tail, return_lse=True)
+        assert torch.equal(o, got[0]) and torch.equal(lse, got[1])

@@ -264,3 +264,19 @@ def test_results_in_one_buffer(layout):
     room = torch.zeros(q.numel(), device="cuda")
     with pytest.raises(ValueError, match="overlap|share storage"):
         ck.apply_rotary(q, k, room.view(torch.int64)[:T], freq, layout=layout, out=(room.view(q.shape), torch.empty_like(k)))
+
+
+def test_yarn_ramp():
+    """Every pair's frequency: theta (1 - r) + theta / s r, r rising from the pair that turns beta_fast times to the one
+    that turns beta_slow times within the trained range (their indices rounded outwards)."""
+    ck = pkg()
+    for rd, base, s, L, fast, slow in ((128, 10000.0, 8.0, 4096, 32.0, 1.0), (64, 500000.0, 4.0, 8192, 16.0, 2.0)):
+        freq, factor = ck.rotary_frequencies(rd, base, "yarn", s, L, beta_fast=fast, beta_slow=slow)
+        assert factor == pytest.approx(0.1 * math.log(s) + 1)
+        at = [rd / 2 * math.log(L / (2 * math.pi * t)) / math.log(base) for t in (fast, slow)]
+        lo, hi = math.floor(at[0]), math.ceil(at[1])
+        assert 0 < lo < hi < rd // 2
+        for i, f in enumerate(theta_of(freq).tolist()):
+            r = min(max((i - lo) / (hi - lo), 0.0), 1.0)
+            theta = base ** (-2 * i / rd)
+            assert f == pytest.approx(theta * (1 - r) + theta / s * r, rel=1e-12)

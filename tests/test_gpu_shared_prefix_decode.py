@@ -385,3 +385,65 @@ def test_layer_calls_refuse_a_prefix_before_the_cache_is_written(pkg):
         with pytest.raises(ValueError, match="SharedPrefix"):
             layer.decode_step_batch(cache, hid[:, 0], prefix=sp)
         assert cache.total_valid_tokens(0, 0) == 0
+
+
+@pytest.mark.parametrize("mode", ["exact", "linear"])
+def test_log_sum_exp_of_the_cached_router(pkg, mode):
+    """The router of the reference's decode step: base sum under the linear correction, shifted logits under the exact."""
+    from oracle.legacy_router import legacy_correction
+    from oracle import unpack_4bit
+    D, Hq, Hkv, T = 64, 4, 2, 150
+    grp = Hq // Hkv
+    with env(**dict(PAPER_BEST_ENV, CAREKV_K_CORRECTION_MODE=mode, CAREKV_KSCORE_LIVE="0")):
+        cfg = pkg.CacheConfig(num_layers=1, num_heads=Hq, num_kv_heads=Hkv, head_dim=D, max_pages=T // 16 + 4,
+                              base_bits=3, group_size=32, scale_quant="int8", store_budget_mode="absolute",
+                              store_abs_k=2, store_abs_v=2, read_budget_mode="absolute", read_abs_k=2, read_abs_v=2,
+                              route_policy="joint", sketch_dim=32, correction_impl="cached")
+        cache = pkg.CAREKVCache(cfg, torch.device("cuda"), batch=1)
+        eng = pkg.DecodeEngine(cache)
+        rng = np.random.default_rng(17)
+        K = rng.standard_normal((Hkv, T, D)).astype(np.float32)
+        K[:, :, :4] *= 20.0
+        V = rng.standard_normal((Hkv, T, D)).astype(np.float32)
+        eng.prefill_store(0, torch.from_numpy(K).cuda()[None], torch.from_numpy(V).cuda()[None])
+        oc = oracle_cache_for(cfg)
+        for h in range(Hkv):
+            oc.prefill_write(0, h, K[h], V[h], "fp32")
+        rc = oracle.RouteConfig(head_dim=D, kind="both", route_policy="joint", score_normalize=True,
+                                k_correction_mode=mode, read_budget_mode="absolute", read_abs_k=2, read_abs_v=2,
+                                read_budget_ratio=0.0)
+        q = rng.standard_normal((Hq, D)).astype(np.float32)
+        qt = torch.from_numpy(q).cuda()[None]
+        plain = eng.attend(0, qt, router="cached")
+        out, lse = eng.attend(0, qt, router="cached", return_lse=True)
+        assert torch.equal(out, plain)
+        sel = eng.last_selection(0, 0, 1, eng._pages(0, 0))
+        lse = lse[0].double().cpu().numpy()
+        checked = 0
+        for h in range(Hkv):
+            K_hat, V_hat, _ = oc.read_base_concat(0, h)
+            for i in range(grp):
+                qi = q[h * grp + i]
+                S, A, O = oracle.base_attention(K_hat, V_hat, qi[None], D)
+                _, info = legacy_correction(oc, 0, h, qi, S[0], A[0], O[0], V_hat, rc, oc.sketch_P, kind="both",
+                                            score_normalize=True, k_corr_scale=0.1, exact=mode == "exact",
+                                            baseline="carekv", rel_thr=0.0, abs_thr=0.0, min_keep=0)
+                want_sel = [("K", p, g) for p, g, _ in info["k_sel"]] + [("V", p, b) for p, b, _ in info["v_sel"]]
+                if sorted(sel[(0, h, i)]) != sorted(want_sel):
+                    continue     # a tie within rounding
+                s = S[0].astype(np.float64)
+                if mode == "exact":
+                    for pid, cg, slot in info["k_sel"]:
+                        p0 = pid * cfg.page_size
+                        p1 = min(p0 + cfg.page_size, T)
+                        packed, sc = oc.read_k_slot(slot)
+                        R = unpack_4bit(packed, sc, cfg.page_size * cfg.k_channel_group)
+                        R = R.reshape(cfg.page_size, cfg.k_channel_group)[:p1 - p0].astype(np.float64)
+                        c0 = cg * cfg.k_channel_group
+                        s[p0:p1] += R @ qi[c0:c0 + cfg.k_channel_group] / math.sqrt(D)
+                m = s.max()
+                want = m + math.log(np.exp(s - m).sum())
+                assert abs(lse[h * grp + i] - want) <= LSE_TOL + 1e-5 * abs(want), (h, i)
+                checked += 1
+        assert checked >= Hq - 1
+        cache.check_errors()

@@ -302,3 +302,19 @@ def test_more_rows_than_one_launch_takes(dtype, rows):
     packed, scale, w = weight(5, 32, 32, dtype, 41)
     x = torch.randn(rows, 32, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(DT[dtype])
     check(ck.PackedWeight(packed, scale, 32).matvec(x), x, w, dtype)
+
+
+def test_results_repeat_and_run_in_a_graph():
+    ck = pkg()
+    for n, k, m in ((250, 768, 3), (3001, 2912, 40), (8209, 4128, 20)):
+        packed, scale, w = weight(n, k, 32, "bf16", 50)
+        pw = ck.PackedWeight(packed, scale, 32)
+        x = torch.randn(m, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(torch.bfloat16)
+        want = pw.matvec(x)
+        for _ in range(20):
+            assert torch.equal(pw.matvec(x), want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = pw.matvec(x)
+        graph.replay()
+        assert torch.equal(y, want)
