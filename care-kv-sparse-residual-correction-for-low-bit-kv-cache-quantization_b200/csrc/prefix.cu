@@ -71,7 +71,7 @@ __device__ __forceinline__ int visible(const PrefixArgs& a, int r) {
 // and 128, rows that do not start on 16-byte boundaries.  A warp per row; the
 // CTA's 8 rows share 32-token tiles of K and V; grid.z splits the prefix.
 // Bound by shared-memory reads, about one word per multiply-add: 16 rows x 32
-// heads of 128 on 32768 tokens of 8 kv heads 4.0 ms, 2.1 TFLOP/s, where the
+// heads of 128 on 32768 tokens of 8 kv heads 4.1 ms, 2.1 TFLOP/s, where the
 // tensor-core form takes 27 us.
 constexpr int kFmaRows = 8, kFmaTok = 32, kFmaMaxD = 256;
 
@@ -149,13 +149,17 @@ __global__ void __launch_bounds__(kFmaRows * 32) prefix_fma_kernel(const PrefixA
 // where m is kept 2^7 low so that small weights stay normal numbers) and the
 // weight sum is kept in fp32 from the unrounded weights.  Rounding P to the
 // 16-bit type of V is what the matrix instruction takes: an error of half an
-// ulp per weight, independent between tokens, like the result's own rounding.
-// Measured: 64 rows x 40 heads of 128 on 8191 tokens of 40 kv heads 40.5 us
-// with the join, 4.1 TB/s of K / V (about 4 us until the first bytes arrive,
-// and the join, are what a copy does not have); 2048 rows x 32 heads of 128 on
-// 8192 tokens of 8 kv heads 305 us, 900 TFLOP/s, bound by the chain S ->
-// maximum -> weights -> P V of a stream (the tensor pipe is busy 47% of the
-// time).  Two threads per row, and registers moved to the softmax warps,
+// ulp per weight, independent between tokens, like the result's own rounding
+// (root mean square against 64 bits, relative, where fp32 weights give
+// 1.66e-3 in bf16 and 2.06e-4 in fp16: up to 2.05e-3 and 2.6e-4).  The lazy
+// maximum and the exponentials on the FMA pipe are published techniques.
+// Measured: 64 rows x 40 heads of 128 on 8191 tokens of 40 kv heads 40.8 us a
+// call with the join, 4.1 TB/s of K / V (about 4 us until the first bytes
+// arrive, and the join, are what a copy does not have); 2048 rows x 32 heads of
+// 128 on 8192 tokens of 8 kv heads 305 us a call, 900 TFLOP/s (the kernel alone
+// 256 us when the GPU pauses between calls and its clock stays high), bound by
+// the chain S -> maximum -> weights -> P V of a stream (the tensor pipe is
+// active 51% of the time, issue 38%).  Two threads per row, and registers moved to the softmax warps,
 // lost more to spills than they gained.
 constexpr int kTcThreads = 320, kTcRows = 128, kTcBlock = 128;
 constexpr float kRaise = 8.f;
@@ -356,8 +360,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const PrefixAr
     }
     __syncwarp();
     // With one tile per kv head every K / V byte is read once: it leaves the
-    // L2 first (16 rows on 32768 tokens 29.3 -> 27.0 us).  With several, the
-    // other tiles' CTAs find it there (2048 rows on 8192: 258 against 264 us).
+    // L2 first (16 rows on 32768 tokens 39.6 -> 37.5 us a call).  With several,
+    // the other tiles' CTAs find it there; the policy makes no difference then
+    // (2048 rows on 8192: 283 us with and without).
     const uint64_t policy = l2_evict_first();
     int cnt = 0;
     bool synced = false;

@@ -11,9 +11,11 @@
 // written once) and the positions, so prompts are bound by HBM and single
 // tokens by the launch.
 //
-// Measured: 4 x 4096 tokens of 32 + 8 heads of 128 in bf16 58.9 us, 5.70 TB/s
-// (87% of a plain copy's rate), 3 x 1021 tokens of 40 + 40 heads in fp32 with
-// 96 of 128 channels turned 50.8 us, 4.94 TB/s; one token 2.5 us.  Twice to four times
+// Measured: 4 x 4096 tokens of 32 + 8 heads of 128 in bf16 58.2 us, 5.77 TB/s
+// (88% of a plain copy's rate), 3 x 1021 tokens of 40 + 40 heads in fp32 with
+// 96 of 128 channels turned 50.4 us, 4.98 TB/s (issue active 68% of the time,
+// 84% of the warps resident: what keeps it from a copy's rate is not known);
+// one token 2.5 us.  Twice to four times
 // the tokens per CTA, streaming stores and several rows in flight per thread
 // changed neither by more than 1%.
 //

@@ -253,9 +253,11 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int j) { return j == 0 
 // the tiles of the rows in turn and add their sums in shared memory.  The
 // next tile's loads are issued before the present tile's products;
 // activations come through L1.  Column lanes past the last row repeat row 0
-// (their sums are not stored).  Bound by the conversion of the codes (issue)
-// and, in small weights, by the latency of the loads: 1 row x 13824 x 5120
-// 11.1 us, 3.4 TB/s; 1 x 4096 x 4096 4.2 us; 16 rows x 14336 x 4096 18.4 us.
+// (their sums are not stored).  Bound by the latency of the loads at as many
+// warps as the registers leave room for: with all inputs out of the L2, 1 row
+// x 13824 x 5120 11.6 us, 3.2 TB/s (issue active 49% of the time, 28 warps an
+// SM at most); 1 x 4096 x 4096 4.6 us; 16 rows x 14336 x 4096 22.5 us (issue
+// active 40%, 12 warps an SM at 153 registers).
 template <int DT, int NS, int MT, int RT, int WK>
 __global__ void __launch_bounds__(WK * 32) w4_kernel(const typename Act<DT>::T* __restrict__ x, int64_t ldx, int M,
                                                      const uint4* __restrict__ codes,
@@ -392,9 +394,10 @@ __global__ void __launch_bounds__(WK * 32) w4_kernel(const typename Act<DT>::T* 
 // held by each).  Codes and scales come through shared
 // memory too, by bulk copies several tiles ahead: with the two tiles a thread
 // could hold in registers the loads in flight bounded the kernel (5120 rows
-// of 13824 channels, 64 activation rows: 35.5 us instead of 28.6, which is
-// 1.4 TB/s or 317 TFLOP/s; bound by a tile's conversion and the wait for its
-// products).  The channels are split over the CTAs of a cluster, which add
+// of 13824 channels, 64 activation rows: 35.5 us instead of 28.6; 29.9 with
+// all inputs out of the L2, 1.3 TB/s or 303 TFLOP/s).  Bound by the chain of a
+// group's tile, conversion -> products -> scaled sums, which has one buffer of
+// codes: the tensor pipe is active 19% of the time and issue 32%.  The channels are split over the CTAs of a cluster, which add
 // their sums through distributed shared memory in a fixed order.
 template <int NS, int NT>
 struct TcLayout {
@@ -702,16 +705,16 @@ cudaError_t launch_tc(const carekv_w4_t& w, const void* x, int64_t ldx, int M, v
 }
 // Which form.  Up to 16 rows (any number in fp32) the few-row kernel, with as
 // many warps per 16 weight rows as the number of such panels leaves room for.
-// Measured with 4 / 8 / 16 warps, us per call:
-//   1 row:   864 panels of 5120 channels 11.1 / 11.9 / 13.3, 320 of 13824
-//            18.8 / 13.0 / 15.1, 256 of 4096 5.5 / 4.4 / 4.2
-//   16 rows: 864 panels of 5120 (two panels a CTA with 4 warps) 14.9 / 17.5 /
-//            24.7, 320 of 13824 27.5 / 19.4 / 26.9, 64 of 4096 6.9 / 5.4 / 3.9
+// Measured with 4 / 8 / 16 warps, us on the device, weights out of the L2:
+//   1 row:   864 panels of 5120 channels 11.1 / 11.9 / 13.2, 320 of 13824
+//            18.7 / 13.1 / 13.9, 256 of 4096 7.6 / 5.4 / 4.7
+//   16 rows: 864 panels of 5120 (two panels a CTA with 4 warps) 14.9 / 17.9 /
+//            25.2, 320 of 13824 27.5 / 19.5 / 27.5, 64 of 4096 9.5 / 6.6 / 4.4
 // Beyond 16 rows that kernel reads the weight again for every 16, and the
 // tcgen05 kernel takes over where the weight is large: 32 rows x 14336 x 4096
-// 28.5 against 21.3 us, but 32 x 4096 x 4096 8.5 against 9.6; 64 x 5120 x
-// 13824 56 against 28.6, 40 x 5632 x 2048 11.3 against 11.2, 48 x 700 x 512
-// 2.7 against 9.5.
+// 28.2 against 21.2 us, and the same 10.8 at 32 x 4096 x 4096; 64 x 5120 x
+// 13824 52.3 against 29.6, 64 x 4096 x 4096 19.3 against 15.2, 40 x 5632 x 2048
+// 11.2 against 11.8, 48 x 700 x 512 2.4 against 10.3.
 template <int DT, int NS>
 cudaError_t launch_ns(const carekv_w4_t& w, const void* x, int64_t ldx, int M, void* out, cudaStream_t st) {
   const int panels = (w.n + kTileRows - 1) / kTileRows, sms = sm_count();

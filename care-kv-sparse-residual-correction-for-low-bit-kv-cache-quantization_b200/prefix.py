@@ -37,9 +37,14 @@ def prefix_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = N
     Returns [n, Hq, D] in q's dtype, with return_lse also the merged
     log-sum-exp [n, Hq] fp32; a row that sees nothing gives 0 and -inf.
     Values of a token that any row sees must be finite for every row.
+    fp16 / bf16 with D 64 or 128 run on the tensor cores, with the softmax
+    weights rounded to that type for the product with V; fp32, other D, and
+    q, k, v, out or tail rows that do not start on 16-byte boundaries take an
+    fp32 form that is about 100 times slower on long prefixes.
     There is no backward pass: inputs that require a gradient are refused.
     """
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ((q, k, v) if tail is None else (q, k, v, *tail))):
+    if (q.requires_grad or k.requires_grad or v.requires_grad or (
+            tail is not None and (tail[0].requires_grad or tail[1].requires_grad))) and torch.is_grad_enabled():
         raise RuntimeError("prefix_attention has no backward pass: detach its inputs or call it under no_grad")
     need_cuda(q, "prefix_attention q")
     dt = dtype_code(q, "prefix_attention q")
