@@ -142,25 +142,25 @@ __global__ void __launch_bounds__(kFmaRows * 32) prefix_fma_kernel(const PrefixA
 //    are two tiles of 128 rows that take the same blocks, so a K / V tile in
 //    shared memory serves 256 rows.
 // A block: S = Q K^T (shared x shared), P = 2^(S scale2 - m) from the
-// registers of the row's thread back to TMEM, O += P V (TMEM x shared, V
-// read MN-major from its [token][channel] tile).  The running maximum m is
-// only raised when a block exceeds it by 2^8, so O is rescaled a few times
-// per row and not at every block; the weights stay below 2^8 (2^15 in fp16,
-// where m is kept 2^7 low so that small weights stay normal numbers) and the
-// weight sum is kept in fp32 from the unrounded weights.  Rounding P to the
-// 16-bit type of V is what the matrix instruction takes: an error of half an
-// ulp per weight, independent between tokens, like the result's own rounding
-// (root mean square against 64 bits, relative, where fp32 weights give
-// 1.66e-3 in bf16 and 2.06e-4 in fp16: up to 2.05e-3 and 2.6e-4).  The lazy
-// maximum and the exponentials on the FMA pipe are published techniques.
-// Measured: 64 rows x 40 heads of 128 on 8191 tokens of 40 kv heads 40.8 us a
-// call with the join, 4.1 TB/s of K / V (about 4 us until the first bytes
-// arrive, and the join, are what a copy does not have); 2048 rows x 32 heads of
-// 128 on 8192 tokens of 8 kv heads 305 us a call, 900 TFLOP/s (the kernel alone
-// 256 us when the GPU pauses between calls and its clock stays high), bound by
-// the chain S -> maximum -> weights -> P V of a stream (the tensor pipe is
-// active 51% of the time, issue 38%).  Two threads per row, and registers moved to the softmax warps,
-// lost more to spills than they gained.
+// registers of the row's thread back to TMEM, O += P V (TMEM x shared, V read
+// MN-major from its [token][channel] tile).  The running maximum m is only
+// raised when a block exceeds it by 2^8, so O is rescaled a few times per row
+// and not at every block; the weights stay below 2^8 (2^15 in fp16, where m is
+// kept 2^7 low so that small weights stay normal numbers) and the weight sum
+// is kept in fp32 from the unrounded weights.  Rounding P to the 16-bit type of
+// V is what the matrix instruction takes: an error of half an ulp per weight,
+// independent between tokens, like the result's own rounding (root mean square
+// against 64 bits, relative, where fp32 weights give 1.66e-3 in bf16 and
+// 2.06e-4 in fp16: up to 2.05e-3 and 2.6e-4).  The lazy maximum and the
+// exponentials on the FMA pipe are published techniques.  Measured: 64 rows x
+// 40 heads of 128 on 8191 tokens of 40 kv heads 40.8 us a call with the join,
+// 4.1 TB/s of K / V (about 4 us until the first bytes arrive, and the join,
+// are what a copy does not have); 2048 rows x 32 heads of 128 on 8192 tokens
+// of 8 kv heads 305 us a call, 900 TFLOP/s (the kernel alone 256 us when the
+// GPU pauses between calls and its clock stays high), bound by the chain S ->
+// maximum -> weights -> P V of a stream (the tensor pipe is active 51% of the
+// time, issue 38%).  Two threads per row, and registers moved to the softmax
+// warps, lost more to spills than they gained.
 constexpr int kTcThreads = 320, kTcRows = 128, kTcBlock = 128;
 constexpr float kRaise = 8.f;
 // One of so many pairs of weights is computed on the FMA pipe: the 16

@@ -15,9 +15,8 @@
 // (88% of a plain copy's rate), 3 x 1021 tokens of 40 + 40 heads in fp32 with
 // 96 of 128 channels turned 50.4 us, 4.98 TB/s (issue active 68% of the time,
 // 84% of the warps resident: what keeps it from a copy's rate is not known);
-// one token 2.5 us.  Twice to four times
-// the tokens per CTA, streaming stores and several rows in flight per thread
-// changed neither by more than 1%.
+// one token 2.5 us.  Twice to four times the tokens per CTA, streaming stores
+// and several rows in flight per thread changed neither by more than 1%.
 //
 // A CTA takes ktok tokens: its threads first put the tokens' cos / sin in
 // shared memory (one pair each), then walk the tokens' heads with 16-byte

@@ -378,27 +378,28 @@ __global__ void __launch_bounds__(WK * 32) w4_kernel(const typename Act<DT>::T* 
   }
 }
 
-// More rows (up to NT = 32 or 64, 16-bit) on tcgen05: a CTA takes 128
-// weight rows, the M side of the instruction, against the NT activation rows
-// of its N side.  A thread owns a weight row: it turns the row's 128 codes of
-// a tile into 16-bit numbers in 64 columns of its TMEM lane, from where the
+// More rows (up to NT = 32 or 64, 16-bit) on tcgen05: a CTA takes 128 weight
+// rows, the M side of the instruction, against the NT activation rows of its N
+// side.  A thread owns a weight row: it turns the row's 128 codes of a tile
+// into 16-bit numbers in 64 columns of its TMEM lane, from where the
 // instruction reads them as operand A, so the dequantized weight never passes
 // through shared memory (2 bytes per code written and read back there would
 // bound the kernel below HBM speed); the activations' tile is operand B, by
 // TMA.  Each scale group has a product sum of its own in TMEM, which the row's
 // thread multiplies by its scale and adds in fp32 registers: weights stay
-// exact.  Groups of four warps take the tiles in turn, each converting,
-// issuing its products (one warp issuing for all took 0.5 us a tile), waiting
-// for them and adding by itself; what hides the waits is the other groups'
-// work, so there are as many as the registers allow (the NT sums of a row are
-// held by each).  Codes and scales come through shared
-// memory too, by bulk copies several tiles ahead: with the two tiles a thread
-// could hold in registers the loads in flight bounded the kernel (5120 rows
-// of 13824 channels, 64 activation rows: 35.5 us instead of 28.6; 29.9 with
-// all inputs out of the L2, 1.3 TB/s or 303 TFLOP/s).  Bound by the chain of a
-// group's tile, conversion -> products -> scaled sums, which has one buffer of
-// codes: the tensor pipe is active 19% of the time and issue 32%.  The channels are split over the CTAs of a cluster, which add
-// their sums through distributed shared memory in a fixed order.
+// exact.  Groups of four warps take the tiles in turn, each converting, issuing
+// its products (one warp issuing for all took 0.5 us a tile), waiting for them
+// and adding by itself; what hides the waits is the other groups' work, so
+// there are as many as the registers allow (the NT sums of a row are held by
+// each).  Codes and scales come through shared memory too, by bulk copies
+// several tiles ahead: with the two tiles a thread could hold in registers the
+// loads in flight bounded the kernel (5120 rows of 13824 channels, 64
+// activation rows: 35.5 us instead of 28.6; 29.9 with all inputs out of the
+// L2, 1.3 TB/s or 303 TFLOP/s).  Bound by the chain of a group's tile,
+// conversion -> products -> scaled sums, which has one buffer of codes: the
+// tensor pipe is active 19% of the time and issue 32%.  The channels are split
+// over the CTAs of a cluster, which add their sums through distributed shared
+// memory in a fixed order.
 template <int NS, int NT>
 struct TcLayout {
   static constexpr int kStages = NT == 64 ? 6 : 8;
